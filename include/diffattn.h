@@ -38,7 +38,8 @@ enum {
   DIFFATTN_ERR_WORKSPACE = -8,      /* workspace missing or too small */
   DIFFATTN_ERR_CUDA = -9,           /* a CUDA runtime/driver call failed */
   DIFFATTN_ERR_TIMEOUT = -10,       /* a device-side wait gave up (reported by diffattn_status) */
-  DIFFATTN_ERR_WRONG_DEVICE = -11   /* a tensor pointer is not device memory of `device` (host memory, another GPU) */
+  DIFFATTN_ERR_WRONG_DEVICE = -11,  /* a tensor pointer is not device memory of `device` (host memory, another GPU) */
+  DIFFATTN_ERR_BAD_CACHE = -12      /* a length, a page or a full cache that a kernel met (reported by diffattn_status) */
 };
 
 enum { DIFFATTN_LAMBDA_F16 = 0, DIFFATTN_LAMBDA_F32 = 1, DIFFATTN_LAMBDA_BF16 = 2 };
@@ -153,6 +154,72 @@ int diffattn_lambda_fwd(int32_t device, void* stream, int32_t n, const float* q1
                         float lambda_init, float* out);
 int diffattn_lambda_bwd(int32_t device, void* stream, int32_t n, const float* q1, const float* k1, const float* q2, const float* k2,
                         const float* out, const float* dlambda, float* dq1, float* dk1, float* dq2, float* dk2);
+
+/* ---- Key-value cache: generation, one token at a time (no counterpart in the reference, which trains only) ----
+ *
+ * Pages of page_size slots; the rows of all heads lie in a page: k1_pages, k2_pages [num_pages][H][page_size][D] with one set of element
+ * strides, v_pages [num_pages][H][page_size][2D] with its own (any order of the three outer dimensions; last dimension contiguous, strides
+ * positive multiples of 8 elements, bases 16-byte aligned).  Slot j of sequence b lies in slot j % page_size of page
+ * page_table[b * table_stride + j / page_size]; a sequence can hold slots = max_pages * page_size tokens.  Row types: io_dtype.
+ * lengths [B]: tokens that each sequence holds, in slots 0 .. lengths[b] - 1; 0 is a sequence that is not in use.  next_position [B]: tokens
+ * it has had.  positions [B][H][slots]: the position of the token in each slot (per head: heads lose different tokens).  weights
+ * [B][H][slots]: the attention weight that each token has gathered, sum of |P_1 - lambda P_2| over the queries that saw it.  positions and
+ * next_position go together; they and weights may be NULL where nothing is evicted.  Slots behind a sequence's length are never
+ * read, and written only by append.
+ *
+ * Lengths and pages lie on the device, so the kernels check them: a length outside [0, slots] counts as the nearest bound, a page
+ * outside [0, num_pages) is neither read nor written, tokens that do not fit are dropped; the results of such a call are undefined,
+ * and diffattn_status reports it as DIFFATTN_ERR_BAD_CACHE.  Pages may be shared between sequences (a common prefix) as long as the slots
+ * that a call writes belong to one sequence: the one behind each length (append, attend with a token), all of a sequence longer than
+ * `keep` (evict).  B <= 4096, B * H <= 65535, slots + page_size < 2^31.  Calls are enqueued on `stream`, allocate nothing and can be captured. */
+typedef struct DiffAttnCacheParams {
+  uint32_t struct_size;            /* sizeof(DiffAttnCacheParams) */
+  int32_t device;
+  void* stream;                    /* cudaStream_t */
+  int32_t B, H, D;
+  int32_t io_dtype;                /* DIFFATTN_IO_*: pages, new tokens, queries, y */
+  int32_t page_size, num_pages, max_pages;
+  int32_t T;                       /* append: rows per (sequence, head) of k1, k2, v */
+  int64_t kp_stride_page, kp_stride_head, kp_stride_slot;         /* in elements */
+  int64_t vp_stride_page, vp_stride_head, vp_stride_slot;
+  void* k1_pages; void* k2_pages; void* v_pages;
+  const int32_t* page_table;
+  int64_t table_stride;            /* in elements */
+  int32_t* lengths; int32_t* next_position; int32_t* positions; float* weights;
+  /* new tokens: append [B, H, T, D] / [.., 2D]; attend [B, H, D] / [.., 2D] (the t strides are not read) or all NULL */
+  const void* k1; const void* k2; const void* v;
+  int64_t k_stride_b, k_stride_h, k_stride_t;
+  int64_t v_stride_b, v_stride_h, v_stride_t;
+  const int32_t* counts;           /* append: [B] rows that each sequence gets (0 .. T), or NULL: T */
+  /* attend */
+  const void* q1; const void* q2;  /* [B, H, D], one set of strides */
+  int64_t q_stride_b, q_stride_h;
+  const void* lambda_scale;        /* as in DiffAttnParams */
+  int32_t lambda_dtype, rms_norm;
+  float sm_scale, lambda_init, eps;
+  int32_t keep;                    /* evict: tokens that stay per (sequence, head), 1 .. slots */
+  const float* gain;               /* [2D] or NULL */
+  void* y;                         /* [B, H, 2D] dense */
+  int32_t recent;                  /* evict: tokens of the last `recent` positions stay, 0 .. keep */
+  int32_t reserved;
+  void* workspace;                 /* diffattn_cache_workspace_bytes(), 256-byte aligned */
+  uint64_t workspace_bytes;
+} DiffAttnCacheParams;
+
+enum { DIFFATTN_CACHE_APPEND = 0, DIFFATTN_CACHE_ATTEND = 1, DIFFATTN_CACHE_EVICT = 2 };
+
+/* Stores k1, k2, v behind each sequence's last token (positions follow on, weights start at 0) and moves lengths and next_position on. */
+int diffattn_cache_append(const DiffAttnCacheParams* p);
+/* y = (softmax(s q1 K1^T) - lambda softmax(s q2 K2^T)) V, norm and gain as diffattn_fwd, for one query per (sequence, head) over the
+ * sequence's tokens; y = 0 where it has none.  With k1, k2, v (one token per sequence) that token is stored first, as append
+ * does, and takes part.  weights, where given, grow by |P_1 - lambda P_2|.  Bit-reproducible on a given GPU model. */
+int diffattn_cache_attend(const DiffAttnCacheParams* p);
+/* Cuts every sequence longer than `keep` back to `keep` tokens, per head: those of the last `recent` positions stay, then those
+ * with the largest weights (ties: the lowest slot; NaN counts as the largest), without weights those of the largest positions.  Survivors in slots
+ * >= keep move into the slots that come free below, in slot order.  Needs positions and next_position. */
+int diffattn_cache_evict(const DiffAttnCacheParams* p);
+/* Scratch bytes that an operation (DIFFATTN_CACHE_*) needs for these sizes: nothing in it has to be initialised or survives the call. */
+uint64_t diffattn_cache_workspace_bytes(const DiffAttnCacheParams* p, int32_t operation);
 
 /* Scratch bytes diffattn_bwd needs for these shapes and p->single_pass (the reference allocates its
  * D1/D2 and dLambda partial buffers itself, src/kernel.py:522-529).  The forward needs none. */

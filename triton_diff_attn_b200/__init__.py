@@ -3,8 +3,9 @@
 libdiffattn.so and raises if it has not been built; there is no fallback path."""
 from .layers import (DiffAttnCore, DiffAttnFunction, MultiheadDiffAttnKernel, device_status,  # noqa: F401
                      lambda_from_reparam)
+from .cache import DiffAttnCache  # noqa: F401
 from .host_pipeline import HostStepPipeline  # noqa: F401
 from .shard import shard_range, shard_batch, sum_dlambda_on_host  # noqa: F401
 
 __all__ = ["MultiheadDiffAttnKernel", "DiffAttnFunction", "device_status", "shard_range", "shard_batch",
-           "sum_dlambda_on_host", "HostStepPipeline", "lambda_from_reparam", "DiffAttnCore"]
+           "sum_dlambda_on_host", "HostStepPipeline", "lambda_from_reparam", "DiffAttnCore", "DiffAttnCache"]

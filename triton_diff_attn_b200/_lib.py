@@ -13,13 +13,14 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("DIFFATTN_LIBRARY") or os.path.join(PKG_DIR, "libdiffattn.so")
 
 EXPORTS = ("diffattn_fwd", "diffattn_bwd", "diffattn_bwd_stages", "diffattn_bwd_static", "diffattn_lambda_fwd", "diffattn_lambda_bwd", "diffattn_workspace_bytes", "diffattn_status",
-           "diffattn_last_error", "diffattn_version", "diffattn_supports")
+           "diffattn_last_error", "diffattn_version", "diffattn_supports",
+           "diffattn_cache_append", "diffattn_cache_attend", "diffattn_cache_evict", "diffattn_cache_workspace_bytes")
 
 ERR_NAMES = {
     0: "OK", -1: "NULL_PTR", -2: "BAD_STRUCT", -3: "BAD_SHAPE", -4: "UNSUPPORTED_D", -5: "BAD_STRIDE",
-    -6: "MISALIGNED", -7: "BAD_DTYPE", -8: "WORKSPACE", -9: "CUDA", -10: "TIMEOUT", -11: "WRONG_DEVICE",
+    -6: "MISALIGNED", -7: "BAD_DTYPE", -8: "WORKSPACE", -9: "CUDA", -10: "TIMEOUT", -11: "WRONG_DEVICE", -12: "BAD_CACHE",
 }
-VALUE_ERRORS = (-1, -2, -3, -4, -5, -6, -7, -8, -11)   # caller mistakes -> ValueError; the rest RuntimeError
+VALUE_ERRORS = (-1, -2, -3, -4, -5, -6, -7, -8, -11, -12)   # caller mistakes -> ValueError; the rest RuntimeError
 
 LAMBDA_F16, LAMBDA_F32, LAMBDA_BF16 = 0, 1, 2
 IO_F16, IO_BF16 = 0, 1
@@ -47,6 +48,32 @@ class DiffAttnParams(C.Structure):
     ]
 
 
+CACHE_APPEND, CACHE_ATTEND, CACHE_EVICT = 0, 1, 2
+
+
+class DiffAttnCacheParams(C.Structure):
+    """Mirror of `struct DiffAttnCacheParams` (include/diffattn.h); field order and types must match."""
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("device", C.c_int32), ("stream", C.c_void_p),
+        ("B", C.c_int32), ("H", C.c_int32), ("D", C.c_int32), ("io_dtype", C.c_int32),
+        ("page_size", C.c_int32), ("num_pages", C.c_int32), ("max_pages", C.c_int32), ("T", C.c_int32),
+        ("kp_stride_page", C.c_int64), ("kp_stride_head", C.c_int64), ("kp_stride_slot", C.c_int64),
+        ("vp_stride_page", C.c_int64), ("vp_stride_head", C.c_int64), ("vp_stride_slot", C.c_int64),
+        ("k1_pages", C.c_void_p), ("k2_pages", C.c_void_p), ("v_pages", C.c_void_p),
+        ("page_table", C.c_void_p), ("table_stride", C.c_int64),
+        ("lengths", C.c_void_p), ("next_position", C.c_void_p), ("positions", C.c_void_p), ("weights", C.c_void_p),
+        ("k1", C.c_void_p), ("k2", C.c_void_p), ("v", C.c_void_p),
+        ("k_stride_b", C.c_int64), ("k_stride_h", C.c_int64), ("k_stride_t", C.c_int64),
+        ("v_stride_b", C.c_int64), ("v_stride_h", C.c_int64), ("v_stride_t", C.c_int64),
+        ("counts", C.c_void_p),
+        ("q1", C.c_void_p), ("q2", C.c_void_p), ("q_stride_b", C.c_int64), ("q_stride_h", C.c_int64),
+        ("lambda_scale", C.c_void_p), ("lambda_dtype", C.c_int32), ("rms_norm", C.c_int32),
+        ("sm_scale", C.c_float), ("lambda_init", C.c_float), ("eps", C.c_float), ("keep", C.c_int32),
+        ("gain", C.c_void_p), ("y", C.c_void_p), ("recent", C.c_int32), ("reserved", C.c_int32),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
+    ]
+
+
 def _load() -> C.CDLL:
     if not os.path.exists(LIB_PATH):
         raise ImportError(
@@ -68,6 +95,13 @@ def _load() -> C.CDLL:
         lib.diffattn_lambda_fwd.restype = C.c_int
         lib.diffattn_lambda_bwd.argtypes = [C.c_int32, C.c_void_p, C.c_int32] + [C.c_void_p] * 10
         lib.diffattn_lambda_bwd.restype = C.c_int
+    lib.has_cache = all(hasattr(lib, "diffattn_cache_" + name) for name in ("append", "attend", "evict", "workspace_bytes"))
+    if lib.has_cache:
+        for fn in (lib.diffattn_cache_append, lib.diffattn_cache_attend, lib.diffattn_cache_evict):
+            fn.argtypes = [C.POINTER(DiffAttnCacheParams)]
+            fn.restype = C.c_int
+        lib.diffattn_cache_workspace_bytes.argtypes = [C.POINTER(DiffAttnCacheParams), C.c_int32]
+        lib.diffattn_cache_workspace_bytes.restype = C.c_uint64
     lib.diffattn_workspace_bytes.argtypes = [C.POINTER(DiffAttnParams)]
     lib.diffattn_workspace_bytes.restype = C.c_uint64
     lib.diffattn_status.argtypes = [C.c_int32]

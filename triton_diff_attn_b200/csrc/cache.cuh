@@ -1,0 +1,133 @@
+// Paged key-value cache of differential attention: what its kernels share, and the kernels that store new tokens.
+//
+// A sequence's token j lies in slot j % page_size of page page_table[b][j / page_size]; a page holds the rows of all heads.  Rows: K1, K2 of
+// D, V of 2D 16-bit elements, 8 D bytes a token and head.  Nothing about a sequence is known on the host but the table's width, so lengths
+// and pages are checked here: a length outside [0, slots] counts as the nearest bound, a page outside the pool is not touched, and
+// both are reported through the status word.
+#pragma once
+#include "sm100.cuh"
+
+namespace da {
+
+// what g_status[0] holds for a cache whose contents make no sense (sites of waits that gave up are below)
+constexpr int kCacheSite = 900;
+constexpr int kCacheBadLength = 901, kCacheBadPage = 902, kCacheFull = 903;
+
+__device__ __noinline__ void cache_fault(int site, int b, int at) {
+  if (atomicCAS(&g_status[0], 0, site) == 0) {
+    g_status[1] = b;
+    g_status[2] = at;
+    g_status[3] = 0;
+  }
+}
+
+struct CacheArgs {
+  int b, h;
+  int page_size, max_pages, num_pages;
+  int slots;                         // page_size * max_pages: what a sequence can hold
+  uint32_t page_magic;               // ceil(2^32 / page_size); 0: pages of one slot
+  const int* page_table;             // [b][max_pages], rows table_stride apart
+  long long table_stride;
+  int* lengths;                      // [b]
+  int* next_position;                // [b] or null: tokens that the sequence has had, with those evicted
+  int* positions;                    // [b][h][slots] or null: the position of the token in each slot
+  float* weights;                    // [b][h][slots] or null: accumulated attention weights
+  uint4* k1; uint4* k2; uint4* v;    // the pools; strides in 16-byte pieces
+  long long k_page, k_head, k_slot;
+  long long v_page, v_head, v_slot;
+};
+
+__device__ __forceinline__ int cache_length(const CacheArgs& c, int b) {
+  const int n = c.lengths[b];
+  if (n >= 0 && n <= c.slots) return n;
+  cache_fault(kCacheBadLength, b, n);
+  return n < 0 ? 0 : c.slots;
+}
+// slot / page_size: slot < 2^31 and page_magic - 2^32 / page_size < 1, so the product is at most one quotient too high
+__device__ __forceinline__ int cache_page(const CacheArgs& c, int slot) {
+  int p = c.page_magic ? int(__umulhi(uint32_t(slot), c.page_magic)) : slot;
+  if ((long long)p * c.page_size > slot) --p;
+  return p;
+}
+// the page behind entry `i` of sequence b's table, or -1
+__device__ __forceinline__ int cache_page_id(const CacheArgs& c, int b, int i) {
+  const int id = __ldg(c.page_table + b * c.table_stride + i);
+  if (uint32_t(id) < uint32_t(c.num_pages)) return id;
+  cache_fault(kCacheBadPage, b, i);
+  return -1;
+}
+
+// The 16-byte piece `part` (of D / 2: K1, then K2, then V) of a cached row.
+template <int D>
+__device__ __forceinline__ uint4* cache_piece(const CacheArgs& c, int page, int head, int in_page, int part) {
+  constexpr int KP = D / 8;
+  if (part < 2 * KP) return (part < KP ? c.k1 : c.k2) + page * c.k_page + head * c.k_head + in_page * c.k_slot + (part & (KP - 1));
+  return c.v + page * c.v_page + head * c.v_head + in_page * c.v_slot + (part - 2 * KP);
+}
+
+struct CacheAppendArgs {
+  CacheArgs c;
+  int t;                             // rows given per (sequence, head)
+  const int* counts;                 // [b] or null (all t): how many of them sequence b gets
+  const uint4* k1; const uint4* k2; const uint4* v;
+  long long k_b, k_h, k_t, v_b, v_h, v_t;      // in 16-byte pieces
+};
+
+__device__ __forceinline__ int append_count(const CacheAppendArgs& a, int b) { return a.counts ? min(max(a.counts[b], 0), a.t) : a.t; }
+
+// Stores new rows behind each sequence's last one.  Bound by HBM: 8 D bytes in and out per row.  A thread moves 16-byte pieces, neighbours
+// along a row, four rows' pieces in flight; grid (rows, b * h).
+constexpr int APPEND_THREADS = 256, APPEND_UNROLL = 4;
+
+template <int D>
+__global__ void __launch_bounds__(APPEND_THREADS) diffattn_cache_append_kernel(const CacheAppendArgs a) {
+  constexpr int PARTS = D / 2, ROWS = APPEND_THREADS / PARTS;
+  const CacheArgs& c = a.c;
+  griddep_launch();
+  const int head = blockIdx.y % c.h, b = blockIdx.y / c.h;
+  const int part = threadIdx.x % PARTS;
+  const int t0 = blockIdx.x * (ROWS * APPEND_UNROLL) + threadIdx.x / PARTS;
+  const int len = cache_length(c, b), count = append_count(a, b);
+  const uint4* src;
+  long long step;
+  if (part < D / 4) {
+    src = (part < D / 8 ? a.k1 : a.k2) + b * a.k_b + head * a.k_h + (part & (D / 8 - 1));
+    step = a.k_t;
+  } else {
+    src = a.v + b * a.v_b + head * a.v_h + (part - D / 4);
+    step = a.v_t;
+  }
+  uint4 x[APPEND_UNROLL];
+#pragma unroll
+  for (int i = 0; i < APPEND_UNROLL; ++i)
+    if (t0 + i * ROWS < count) x[i] = __ldg(src + (t0 + i * ROWS) * step);
+#pragma unroll
+  for (int i = 0; i < APPEND_UNROLL; ++i) {
+    const int t = t0 + i * ROWS;
+    if (t >= count) break;
+    if (t >= c.slots - len) {
+      cache_fault(kCacheFull, b, len);
+      break;
+    }
+    const int slot = len + t, p = cache_page(c, slot);
+    const int page = cache_page_id(c, b, p);
+    if (page >= 0) *cache_piece<D>(c, page, head, slot - p * c.page_size, part) = x[i];
+    if (part == 0) {
+      const long long at = (long long)blockIdx.y * c.slots + slot;
+      if (c.positions) c.positions[at] = c.next_position[b] + t;
+      if (c.weights) c.weights[at] = 0.f;
+    }
+  }
+}
+
+// The lengths move on once every row is stored (the kernel above reads them).
+__global__ void __launch_bounds__(APPEND_THREADS) diffattn_cache_advance_kernel(const CacheAppendArgs a) {
+  griddep_wait();
+  const int b = blockIdx.x * APPEND_THREADS + threadIdx.x;
+  if (b >= a.c.b) return;
+  const int len = cache_length(a.c, b), stored = min(append_count(a, b), a.c.slots - len);
+  a.c.lengths[b] = len + stored;
+  if (a.c.next_position) a.c.next_position[b] += stored;
+}
+
+}  // namespace da

@@ -16,6 +16,8 @@
 #include "bwd.cuh"
 #include "bwd128.cuh"
 #include "bwd_fused64.cuh"
+#include "cache_attend.cuh"
+#include "cache_evict.cuh"
 #include "fwd.cuh"
 #include "fwd64.cuh"
 #include "fwd128.cuh"
@@ -84,10 +86,10 @@ PFN_cuTensorMapEncodeTiled_v12000 get_encode() {
 struct MapKey {
   const void* base;
   int64_t s_row, s2, s3;
-  int32_t cols, rows, d2, d3, box_rows, bf;
+  int32_t cols, rows, d2, d3, box_rows, bf, plain_cols;
   bool operator==(const MapKey& o) const {
     return base == o.base && s_row == o.s_row && s2 == o.s2 && s3 == o.s3 && cols == o.cols && rows == o.rows && d2 == o.d2 &&
-           d3 == o.d3 && box_rows == o.box_rows && bf == o.bf;
+           d3 == o.d3 && box_rows == o.box_rows && bf == o.bf && plain_cols == o.plain_cols;
   }
 };
 struct MapKeyHash {
@@ -97,7 +99,7 @@ struct MapKeyHash {
     mix(uint64_t(k.s_row)); mix(uint64_t(k.s2)); mix(uint64_t(k.s3));
     mix((uint64_t(uint32_t(k.cols)) << 32) | uint32_t(k.rows));
     mix((uint64_t(uint32_t(k.d2)) << 32) | uint32_t(k.d3));
-    mix((uint64_t(uint32_t(k.box_rows)) << 1) | uint32_t(k.bf));
+    mix((uint64_t(uint32_t(k.box_rows)) << 1) | uint32_t(k.bf) | (uint64_t(uint32_t(k.plain_cols)) << 32));
     return size_t(h);
   }
 };
@@ -108,11 +110,12 @@ thread_local std::unordered_map<const void*, int> g_ptr_device;         // base 
 thread_local int g_sm_count[kMaxDevices] = {0};
 
 // 16-bit (fp16, or bf16 when BF) tensor [d3, d2, rows, cols] with element strides (s3, s2, s_row, 1); box = box_rows x 64 columns,
-// 128-byte swizzle (the layout the tcgen05 shared-memory descriptors in sm100.cuh describe).
+// 128-byte swizzle (the layout the tcgen05 shared-memory descriptors in sm100.cuh describe).  plain_cols > 0: box = box_rows x plain_cols, rows
+// one behind the other without a swizzle.
 template <bool BF>
 int make_map(CUtensorMap* map, const void* base, int cols, int rows, int d2, int d3, int64_t s_row, int64_t s2, int64_t s3,
-             int box_rows, const char* what) {
-  const MapKey key{base, s_row, s2, s3, cols, rows, d2, d3, box_rows, BF ? 1 : 0};
+             int box_rows, const char* what, int plain_cols = 0) {
+  const MapKey key{base, s_row, s2, s3, cols, rows, d2, d3, box_rows, BF ? 1 : 0, plain_cols};
   {
     auto it = g_maps.find(key);
     if (it != g_maps.end()) {
@@ -129,9 +132,9 @@ int make_map(CUtensorMap* map, const void* base, int cols, int rows, int d2, int
   if (d3 == 1) strides[2] = strides[1] * cuuint64_t(d2);
   // The box is always 64 columns (128 bytes, one swizzle row).  A tensor narrower than that (head dim 32)
   // is padded by the TMA engine: out-of-range elements arrive as zeros.
-  cuuint32_t box[4] = {64, cuuint32_t(box_rows), 1, 1};
+  cuuint32_t box[4] = {plain_cols ? cuuint32_t(plain_cols) : 64u, cuuint32_t(box_rows), 1, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
-  const CUtensorMapSwizzle sw = CU_TENSOR_MAP_SWIZZLE_128B;
+  const CUtensorMapSwizzle sw = plain_cols ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B;
   CUresult r = enc(map, BF ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
                    CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -551,6 +554,8 @@ int all_stages(const DiffAttnParams* p) {
 
 }  // namespace
 
+#include "cache_host.cuh"      // the cache's entry points: checks, workspace, launches
+
 extern "C" {
 
 int diffattn_fwd(const DiffAttnParams* p) {
@@ -661,6 +666,9 @@ int diffattn_status(int32_t device) {
   if (st[0] != 0) {
     int zero[4] = {0, 0, 0, 0};
     cudaMemcpyToSymbol(da::g_status, zero, sizeof(zero));
+    if (st[0] == da::kCacheBadLength) return fail(DIFFATTN_ERR_BAD_CACHE, "cache: sequence %d has length %d", st[1], st[2]);
+    if (st[0] == da::kCacheBadPage) return fail(DIFFATTN_ERR_BAD_CACHE, "cache: entry %d of sequence %d's page table is no page of the pool", st[2], st[1]);
+    if (st[0] == da::kCacheFull) return fail(DIFFATTN_ERR_BAD_CACHE, "cache: sequence %d is full (length %d), tokens were dropped", st[1], st[2]);
     return fail(DIFFATTN_ERR_TIMEOUT, "device-side wait gave up at site %d (block %d,%d iteration %d)", st[0], st[1], st[2], st[3]);
   }
   return DIFFATTN_OK;
