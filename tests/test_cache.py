@@ -100,58 +100,59 @@ def test_no_cpu_path():
 
 # ---- the walk over tiles, as csrc/cache_attend.cuh and cache_host.cuh have it -------------------------------------------------------------
 def tile_shape(d, page):
-    t = 1024 // d
-    if page < t and t % page == 0 and page * d * 2 % 128 == 0:
-        return t, page, 1
-    return t, t, -(-page // t)
+    t = 32 if d == 32 else 16
+    r = t
+    while page % r:
+        r //= 2
+    return (t, r, 0) if r >= 8 else (t, t, -(-page // t))
 
 
 def tiles_of(n, page, shape, token):
-    t, box, per_page = shape
-    if box < t or per_page == 1:
-        tiles = -(-n // t) if box < t else -(-n // page)
-    else:
-        full = n // page
-        tiles = full * per_page + -(-(n - full * page) // t)
-    return tiles + token
+    t, _, per_page = shape
+    if not per_page:
+        return -(-n // t) + token
+    full = n // page
+    return full * per_page + -(-(n - full * page) // t) + token
 
 
 def tile_at(i, n_tiles, n, page, shape, token):
-    t, box, per_page = shape
+    t, _, per_page = shape
     if token and i == n_tiles - 1:
-        return n, 0, 1, True
-    if box < t:
-        return i * t, 0, min(t, n - i * t), False
-    p = i // per_page
-    in_page = (i - p * per_page) * t
-    slot = p * page + in_page
-    return slot, in_page, min(t, page - in_page, n - slot), False
+        return n, 1, True
+    slot, end = i * t, n
+    if per_page:
+        p = i // per_page
+        slot, end = p * page + (i - p * per_page) * t, min(n, (p + 1) * page)
+    return slot, min(t, end - slot), False
 
 
 @pytest.mark.parametrize("d", [32, 64, 128])
 def test_tiles_cover_every_token_once(d):
     for page in list(range(1, 40)) + [48, 64, 100, 128, 1000]:
         shape = tile_shape(d, page)
-        t, box, _ = shape
-        assert t % box == 0 and (box == t or box * d * 2 % 128 == 0)
+        t, box, per_page = shape
+        assert t % box == 0 and box % 8 == 0           # whole periods of the swizzle
         for n in list(range(0, 3 * t + 2)) + [page - 1, page, page + 1, 4 * page, 4 * page + 1]:
             for token in (0, 1):
                 m, seen = tiles_of(n, page, shape, token), []
                 for i in range(m):
-                    slot, in_page, valid, new = tile_at(i, m, n, page, shape, token)
+                    slot, valid, new = tile_at(i, m, n, page, shape, token)
                     assert 1 <= valid <= t
                     if new:
                         assert slot == n
                         continue
-                    for row in range(valid):           # box row // box, row % box of its page
-                        entry = slot // page + row // box
-                        assert entry * page + in_page + row % box == slot + row and in_page + row % box < page
-                        assert entry <= (n - 1) // page
+                    boxes = [lane for lane in range(32) if lane * box < valid]
+                    assert len(boxes) * box <= t
+                    for row in range(valid):
+                        start = slot + row // box * box          # the box's first slot
+                        entry, in_page = divmod(start, page)
+                        assert row // box in boxes and entry * page + in_page + row % box == slot + row
+                        assert in_page + row % box < page and entry <= (n - 1) // page
                         seen.append(slot + row)
                 assert seen == list(range(n))
         # the bound that the workspace is sized by
         slots = 4 * page
-        most = (-(-slots // t) if box < t else 4 * shape[2]) + 1
+        most = (4 * per_page if per_page else -(-slots // t)) + 1
         assert max(tiles_of(n, page, shape, 1) for n in range(slots + 1)) <= most
 
 

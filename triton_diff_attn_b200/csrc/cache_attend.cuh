@@ -2,8 +2,10 @@
 //
 //   s_b[j] = q_b . k_b[j] / sqrt(D),  P_b = softmax(s_b),  A = P_1 V - lambda P_2 V,  y = A * norm * gain;  w[j] += |P_1[j] - lambda P_2[j]|
 //
-// Bound by HBM: every cached row (8 D bytes) is read once for 12 D flops.  A row meets one query only, so there is no matrix product with
-// more than one row and the tensor cores have nothing to do; fp32 fused multiply-adds in pairs need a third of the issue slots.
+// Bound by HBM: every cached row (8 D bytes) is read once for 12 D flops.  A row meets one query only, so the 128-row tiles of tcgen05 would be
+// 1/128 full; the arithmetic goes through mma.sync with the cached rows as the wide operand, not for its rate but for the instructions that it
+// saves: 16 ldmatrix and 16 mma per 16 tokens at D = 64 where unpacking, fused multiply-adds and sums over lanes took 850
+// instructions and bound the kernel (4.2 TB/s at B8 H8 N8192 D128, issue slots 39 % busy with two warps a scheduler).
 //
 // Split: the tiles of all (sequence, head)s form one line, and every WARP takes an equal, contiguous stretch of it.  Whatever the lengths
 // are, all SMs read the same number of bytes, and nobody waits for anybody: a warp loads its own tiles (TMA, a ring of its own), keeps
@@ -28,8 +30,9 @@ struct AttendArgs {
   float out_scale, eps;
   const float* gain;                           // [2D] or null
   __half* y;                                   // [b][h][2D]
-  int box_rows;                                // rows of one TMA box; several pages make a tile where this is less than a tile
-  int tiles_per_page;                          // 1 where several pages make a tile
+  int box_rows;                                // rows of one TMA box
+  int tiles_per_page;                          // 0: tiles run on over the pages; else a tile stays inside its page
+  uint32_t tiles_magic;                        // ceil(2^32 / tiles_per_page), 0 for 1
   int workers;                                 // warps of the first kernel
   // workspace
   int* prefix;                                 // [b + 1] tiles of the sequences before b, per head
@@ -41,56 +44,83 @@ struct AttendArgs {
 };
 
 namespace attend {
-constexpr int WARPS = 8, THREADS = WARPS * 32;
-constexpr int SLOTS = 3;                       // tiles in flight per warp: 192 KB of requests per SM
 constexpr int MAX_B = 4096;                    // the prefix sums of all sequences lie in shared memory
 template <int D>
 struct Geo {
-  static constexpr int T = 1024 / D;           // tokens per tile: 8 KB of K1, K2, V
-  static constexpr int K_BYTES = T * D * 2, V_BYTES = 2 * K_BYTES, Q_BYTES = 2 * D * 2;
-  static constexpr int SLOT_BYTES = 2 * K_BYTES + V_BYTES + 512;     // the queries of a stretch's first tile lie behind the tile
-  static constexpr int OFF_P = WARPS * SLOTS * SLOT_BYTES;           // probabilities of the current tile, per warp
-  static constexpr int OFF_BAR = OFF_P + WARPS * 2 * T * 4;
-  static constexpr int OFF_PREFIX = OFF_BAR + WARPS * SLOTS * 8 + 16;
-  static constexpr int SMEM = OFF_PREFIX + 16 + THREADS / 32 * 4;    // + 4 (b + 1) bytes of prefix sums
-  static_assert(SMEM + 4 * (MAX_B + 1) + 128 <= 227 * 1024, "shared memory");
+  static constexpr int T = D == 32 ? 32 : 16;  // tokens per tile: 8 KB of K1, K2, V (D = 128: 16 KB)
+  static constexpr int WARPS = D == 128 ? 4 : 8, THREADS = WARPS * 32;
+  static constexpr int SLOTS = 3;              // tiles in flight per warp: 192 KB of requests per SM
+  // a tile in shared memory: boxes of T rows of 128 bytes (K at D = 32: 64 bytes), swizzled by the engine: K1, K2, V
+  static constexpr int K_ROW = D == 32 ? 64 : 128, K_BOXES = D == 128 ? 2 : 1, V_BOXES = D / 32;
+  static constexpr int K_BYTES = T * D * 2, V_BYTES = 2 * K_BYTES, SLOT_BYTES = 2 * K_BYTES + V_BYTES;
+  static constexpr int Q_BYTES = 4 * D;        // the two queries of a (sequence, head), beside its first tile
+  static constexpr int OFF_Q = WARPS * SLOTS * SLOT_BYTES;
+  static constexpr int OFF_BAR = OFF_Q + WARPS * SLOTS * Q_BYTES;
+  static constexpr int OFF_SUM = OFF_BAR + WARPS * SLOTS * 8 + 16;
+  static constexpr int OFF_PREFIX = OFF_SUM + WARPS * 4;
+  static constexpr int SMEM = OFF_PREFIX + 4 + 1024;      // + 4 b bytes of prefix sums; 1024 to align the ring
+  static_assert(SMEM + 4 * MAX_B <= 227 * 1024, "shared memory");
 };
 }  // namespace attend
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// 8 x 8 transpose of 16-bit elements, two per lane (lane / 4: row, lane % 4: pair of columns)
+__device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+  return r;
+}
+// d[16 x 8] += a[16 x 16] b[16 x 8], fp32 sums
+template <bool BF>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (BF)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 
 // A place in the line of tiles: (sequence, head, tile), and the sequence's tiles and cached tokens.
 struct TileWalk {
   int b, h, t, n, len;
 };
 
+__device__ __forceinline__ int divide(int n, int d, uint32_t magic) {      // as cache_page
+  int q = magic ? int(__umulhi(uint32_t(n), magic)) : n;
+  if ((long long)q * d > n) --q;
+  return q;
+}
 template <int T>
 __device__ __forceinline__ int attend_tiles(const AttendArgs& a, int len) {
-  int n;
-  if (a.box_rows < T || a.tiles_per_page == 1) {
-    // several pages per tile (T is a multiple of page_size), or a page per tile
-    n = a.box_rows < T ? (len + T - 1) / T : cache_page(a.c, len + a.c.page_size - 1);
-  } else {
+  int n = (len + T - 1) / T;
+  if (a.tiles_per_page) {
     const int full = cache_page(a.c, len);
     n = full * a.tiles_per_page + (len - full * a.c.page_size + T - 1) / T;
   }
   return n + (a.nk1 != nullptr ? 1 : 0);
 }
-// where a tile's rows begin and how many of them are live; the new token is a tile of its own, the last
+// the slot of a tile's first row and how many of its rows are live; the new token is a tile of its own, the last
 template <int T>
-__device__ __forceinline__ void attend_tile(const AttendArgs& a, int t, int n, int len, int& slot, int& in_page, int& valid, bool& is_new) {
+__device__ __forceinline__ void attend_tile(const AttendArgs& a, int t, int n, int len, int& slot, int& valid, bool& is_new) {
   is_new = a.nk1 != nullptr && t == n - 1;
   if (is_new) {
-    slot = len; in_page = 0; valid = 1;
+    slot = len; valid = 1;
     return;
   }
-  if (a.box_rows < T) {
-    slot = t * T; in_page = 0;
-    valid = min(T, len - slot);
-    return;
+  slot = t * T;
+  int end = len;
+  if (a.tiles_per_page) {
+    const int page = divide(t, a.tiles_per_page, a.tiles_magic);
+    slot = page * a.c.page_size + (t - page * a.tiles_per_page) * T;
+    end = min(len, (page + 1) * a.c.page_size);
   }
-  const int page = a.tiles_per_page == 1 ? t : t / a.tiles_per_page;
-  in_page = (t - page * a.tiles_per_page) * T;
-  slot = page * a.c.page_size + in_page;
-  valid = min(min(T, a.c.page_size - in_page), len - slot);
+  valid = min(T, end - slot);
 }
 __device__ __forceinline__ long long stretch_begin(long long units, int workers, int w) { return units * w / workers; }
 
@@ -123,28 +153,22 @@ __device__ __forceinline__ void walk_next(const AttendArgs& a, const int* prefix
   w.len = length[w.b];
 }
 
-__device__ __forceinline__ f32x2 widen(float2 x) { return pk2(x.x, x.y); }
-
 template <int D, bool BF, bool TRACK>
-__global__ void __launch_bounds__(attend::THREADS, 1)
+__global__ void __launch_bounds__(attend::Geo<D>::THREADS, 1)
 diffattn_cache_attend_kernel(const __grid_constant__ CUtensorMap tm_k1, const __grid_constant__ CUtensorMap tm_k2,
                              const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ AttendArgs a) {
-  using namespace attend;
-  using G = Geo<D>;
-  constexpr int T = G::T;
-  constexpr int LPK = D / 8, LPV = D / 4;      // lanes (16-byte pieces) per K row, per V row
-  constexpr int M1 = LPK / 2, M2 = LPK / 4, M3 = LPK / 8;      // lane bits that select branch and row in the sums over a row's lanes
-  constexpr int NV = LPK < 8 ? 2 : 1;          // scores a lane ends up with
+  using G = attend::Geo<D>;
+  constexpr int T = G::T, WARPS = G::WARPS, SLOTS = G::SLOTS, THREADS = G::THREADS;
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint8_t* ring = smem + warp * (SLOTS * G::SLOT_BYTES);
-  float* prob = reinterpret_cast<float*>(smem + G::OFF_P) + warp * 2 * T;
+  uint8_t* ring_q = smem + G::OFF_Q + warp * (SLOTS * G::Q_BYTES);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + G::OFF_BAR) + warp * SLOTS;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + G::OFF_BAR + WARPS * SLOTS * 8);
   volatile int* drain_flag = abort_flag + 1;
-  int* part_sum = reinterpret_cast<int*>(smem + G::OFF_PREFIX);
-  int* prefix = part_sum + WARPS;
+  int* part_sum = reinterpret_cast<int*>(smem + G::OFF_SUM);
+  int* prefix = reinterpret_cast<int*>(smem + G::OFF_PREFIX);
 
   if (lane == 0) {
     for (int i = 0; i < SLOTS; ++i) mbar_init(&full[i], 1);
@@ -193,69 +217,87 @@ diffattn_cache_attend_kernel(const __grid_constant__ CUtensorMap tm_k1, const __
   const long long first = stretch_begin(units, workers, worker);
   const int count = int(stretch_begin(units, workers, worker + 1) - first);
 
-  // ---- loads.  A tile's boxes: one, or one per page where pages are smaller than a tile; lane i has the page of box i.
+  // ---- loads.  Lane i fetches box i of a tile; its page is looked up one request ahead.
   TileWalk ahead = walk_at(a, prefix, a.c.lengths, first);
   ahead.len = min(max(ahead.len, 0), a.c.slots);
   auto next = [&](TileWalk& w) {
     walk_next(a, prefix, a.c.lengths, w);
     w.len = min(max(w.len, 0), a.c.slots);
   };
-  auto page_ids = [&](const TileWalk& w) {
-    int slot, in_page, valid;
+  struct Box { int page, in_page; };           // page -1: the engine fills the box with zeros; in_page -1: no such box
+  auto look_up = [&](const TileWalk& w) {
+    int slot, valid;
     bool is_new;
-    attend_tile<T>(a, w.t, w.n, w.len, slot, in_page, valid, is_new);
-    int id = 0;
-    if (!is_new && lane * a.box_rows < valid) id = cache_page_id(a.c, w.b, cache_page(a.c, slot) + lane);
-    return id;                                 // (-1: the engine fills the box with zeros)
+    attend_tile<T>(a, w.t, w.n, w.len, slot, valid, is_new);
+    Box x{-1, -1};
+    if (!is_new && lane * a.box_rows < valid) {
+      slot += lane * a.box_rows;
+      const int entry = cache_page(a.c, slot);
+      x.in_page = slot - entry * a.c.page_size;
+      x.page = cache_page_id(a.c, w.b, entry);
+    }
+    return x;
   };
-  auto request = [&](const TileWalk& w, int id, int s, bool with_q) {
-    int slot, in_page, valid;
-    bool is_new;
-    attend_tile<T>(a, w.t, w.n, w.len, slot, in_page, valid, is_new);
+  auto request = [&](const TileWalk& w, const Box& x, int s, bool with_q) {
     uint8_t* at = ring + s * G::SLOT_BYTES;
+    const int boxes = __popc(__ballot_sync(0xffffffffu, x.in_page >= 0));      // 0: the new token
     if (lane == 0) {
-      const int boxes = is_new ? 0 : (valid + a.box_rows - 1) / a.box_rows;
-      mbar_expect_tx(&full[s], (is_new ? 8 * D : boxes * a.box_rows * 8 * D) + (with_q ? G::Q_BYTES : 0));
+      mbar_expect_tx(&full[s], (boxes ? boxes * a.box_rows * 8 * D : 8 * D) + (with_q ? G::Q_BYTES : 0));
       if (with_q) {
-        uint8_t* q = at + 2 * G::K_BYTES + G::V_BYTES;
-        bulk_load_1d(q, a.q1 + w.b * a.q_b + w.h * a.q_h, G::Q_BYTES / 2, &full[s]);
-        bulk_load_1d(q + G::Q_BYTES / 2, a.q2 + w.b * a.q_b + w.h * a.q_h, G::Q_BYTES / 2, &full[s]);
+        bulk_load_1d(ring_q + s * G::Q_BYTES, a.q1 + w.b * a.q_b + w.h * a.q_h, 2 * D, &full[s]);
+        bulk_load_1d(ring_q + s * G::Q_BYTES + 2 * D, a.q2 + w.b * a.q_b + w.h * a.q_h, 2 * D, &full[s]);
       }
-      if (is_new) {
-        bulk_load_1d(at, a.nk1 + w.b * a.nk_b + w.h * a.nk_h, 2 * D, &full[s]);
-        bulk_load_1d(at + G::K_BYTES, a.nk2 + w.b * a.nk_b + w.h * a.nk_h, 2 * D, &full[s]);
-        bulk_load_1d(at + 2 * G::K_BYTES, a.nv + w.b * a.nv_b + w.h * a.nv_h, 4 * D, &full[s]);
+      if (boxes == 0) {
+        // row 0 of every box: the swizzle leaves it as it is
+        for (int i = 0; i < G::K_BOXES; ++i) {
+          bulk_load_1d(at + i * T * G::K_ROW, a.nk1 + w.b * a.nk_b + w.h * a.nk_h + i * 8, G::K_ROW, &full[s]);
+          bulk_load_1d(at + G::K_BYTES + i * T * G::K_ROW, a.nk2 + w.b * a.nk_b + w.h * a.nk_h + i * 8, G::K_ROW, &full[s]);
+        }
+        for (int i = 0; i < G::V_BOXES; ++i) bulk_load_1d(at + 2 * G::K_BYTES + i * T * 128, a.nv + w.b * a.nv_b + w.h * a.nv_h + i * 8, 128, &full[s]);
       }
     }
     __syncwarp();
-    if (!is_new && lane * a.box_rows < valid) {
-      const int off = lane * a.box_rows * 2 * D;
-      tma_load_4d(at + off, &tm_k1, &full[s], 0, in_page, w.h, id);
-      tma_load_4d(at + G::K_BYTES + off, &tm_k2, &full[s], 0, in_page, w.h, id);
-      tma_load_4d(at + 2 * G::K_BYTES + 2 * off, &tm_v, &full[s], 0, in_page, w.h, id);
+    if (x.in_page >= 0) {
+      uint8_t* k = at + lane * a.box_rows * G::K_ROW;
+      uint8_t* v = at + 2 * G::K_BYTES + lane * a.box_rows * 128;
+#pragma unroll
+      for (int i = 0; i < G::K_BOXES; ++i) {
+        tma_load_4d(k + i * T * G::K_ROW, &tm_k1, &full[s], i * 64, x.in_page, w.h, x.page);
+        tma_load_4d(k + G::K_BYTES + i * T * G::K_ROW, &tm_k2, &full[s], i * 64, x.in_page, w.h, x.page);
+      }
+#pragma unroll
+      for (int i = 0; i < G::V_BOXES; ++i) tma_load_4d(v + i * T * 128, &tm_v, &full[s], i * 64, x.in_page, w.h, x.page);
     }
   };
   TileWalk cur = ahead;
-  int id;
+  Box box{-1, -1};
   {
     TileWalk w[SLOTS];
-    int ids[SLOTS];
+    Box x[SLOTS];
 #pragma unroll
     for (int i = 0; i < SLOTS; ++i) {
       w[i] = ahead;
-      ids[i] = i < count ? page_ids(ahead) : 0;
+      if (i < count) x[i] = look_up(ahead);
       if (i + 1 < count) next(ahead);
     }
 #pragma unroll
     for (int i = 0; i < SLOTS; ++i)
-      if (i < count) request(w[i], ids[i], i, i == 0 || w[i].t == 0);
-    id = SLOTS < count ? page_ids(ahead) : 0;
+      if (i < count) request(w[i], x[i], i, i == 0 || w[i].t == 0);
+    if (SLOTS < count) box = look_up(ahead);
   }
 
-  // ---- the stretch
-  f32x2 q[2][4], o[2][4];
-  float m = 0.f, l = 0.f;                      // of this lane's branch (bit M1 of the lane); l: of the scores that this lane had
-  const bool second = lane & M1;
+  // ---- the stretch.  With the rows r = 8 x matrix and columns c of the fragments as mma.sync lays them out:
+  //  scores  S_b[16 tokens x 8] = K_b Q^T, Q^T's columns q1, q1, q2, q2, 0, 0, 0, 0: lane % 4 = 0 has S_1, lane % 4 = 1 has S_2 of tokens lane / 4
+  //          and lane / 4 + 8, the other lanes nothing
+  //  P       a probability as two 16-bit numbers, its rounding and what that left out (bf16: 16 bits, fp16: 22), side by side in columns
+  //          2 b, 2 b + 1: transposed it is the operand of
+  //  output  O^T[16 values x 8] += V^T P^T, columns O_1 (two shares), O_2 (two shares): the same lanes have the same branch
+  const int branch = lane & 3;                 // 0, 1; 2 and 3: none
+  const uint32_t row_k = smem_u32(ring) + (lane & 15) * G::K_ROW, row_v = smem_u32(ring) + 2 * G::K_BYTES + ((lane & 7) + ((lane >> 4) << 3)) * 128;
+  const uint32_t sw_k = D == 32 ? ((lane >> 4) ^ ((lane >> 1) & 3)) << 4 : ((lane >> 4) ^ (lane & 7)) << 4, sw_v = (((lane >> 3) & 1) ^ (lane & 7)) << 4;
+  uint32_t q[D / 16][2];
+  float o[D / 8][4];
+  float m = 0.f, l = 0.f;                      // of this lane's branch; l: of the tokens that this lane had
   int s = 0, phase = 0;
   for (int i = 0; i < count; ++i) {
     if (!mbar_wait_warp(&full[s], phase, abort_flag, 801, i)) {
@@ -266,146 +308,117 @@ diffattn_cache_attend_kernel(const __grid_constant__ CUtensorMap tm_k1, const __
       }
       return;
     }
-    const uint8_t* tile = ring + s * G::SLOT_BYTES;
-    int slot, in_page, valid;
+    int slot, valid;
     bool is_new;
-    attend_tile<T>(a, cur.t, cur.n, cur.len, slot, in_page, valid, is_new);
+    attend_tile<T>(a, cur.t, cur.n, cur.len, slot, valid, is_new);
     if (i == 0 || cur.t == 0) {
-      // a (sequence, head) begins: its queries, scaled so that scores come out in base 2
-      const f32x2 sc = pk2(a.scale_log2, a.scale_log2);
+      // a (sequence, head) begins
+      const int n = lane >> 2;
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(ring_q + s * G::Q_BYTES + (n < 2 ? 0 : 2 * D)) + branch;
 #pragma unroll
-      for (int br = 0; br < 2; ++br) {
-        const uint4 w = *reinterpret_cast<const uint4*>(tile + 2 * G::K_BYTES + G::V_BYTES + br * 2 * D + (lane & (LPK - 1)) * 16);
-        q[br][0] = mul2(widen(unpack2<BF>(w.x)), sc);
-        q[br][1] = mul2(widen(unpack2<BF>(w.y)), sc);
-        q[br][2] = mul2(widen(unpack2<BF>(w.z)), sc);
-        q[br][3] = mul2(widen(unpack2<BF>(w.w)), sc);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) o[br][k] = pk2(0.f, 0.f);
+      for (int k = 0; k < D / 16; ++k) {
+        q[k][0] = n < 4 ? src[k * 8] : 0u;
+        q[k][1] = n < 4 ? src[k * 8 + 4] : 0u;
       }
+#pragma unroll
+      for (int k = 0; k < D / 8; ++k) o[k][0] = o[k][1] = o[k][2] = o[k][3] = 0.f;
       m = -3e38f;                              // (finite: a score of -inf then counts as 0 instead of as not a number)
       l = 0.f;
     }
-    if (is_new && slot < a.c.slots) {
-      // the new token goes into the cache on its way
-      const int p = cache_page(a.c, slot);
-      const int page = cache_page_id(a.c, cur.b, p);
-      for (int part = lane; page >= 0 && part < D / 2; part += 32) {
-        const int off = part < D / 8 ? part * 16 : part < D / 4 ? G::K_BYTES + (part - D / 8) * 16 : 2 * G::K_BYTES + (part - D / 4) * 16;
-        *cache_piece<D>(a.c, page, cur.h, slot - p * a.c.page_size, part) = *reinterpret_cast<const uint4*>(tile + off);
+    if (valid < T) {
+      uint8_t* tile = ring + s * G::SLOT_BYTES;
+      if (is_new && slot < a.c.slots) {
+        // the new token goes into the cache on its way
+        const int entry = cache_page(a.c, slot);
+        const int page = cache_page_id(a.c, cur.b, entry);
+        for (int part = lane; page >= 0 && part < D / 2; part += 32) {
+          const int c = part < D / 8 ? part : part < D / 4 ? part - D / 8 : part - D / 4;      // 16-byte piece of its row; eight to a box
+          const int off = part < D / 4 ? (part < D / 8 ? 0 : G::K_BYTES) + (c >> 3) * T * G::K_ROW : 2 * G::K_BYTES + (c >> 3) * T * 128;
+          *cache_piece<D>(a.c, page, cur.h, slot - entry * a.c.page_size, part) = *reinterpret_cast<const uint4*>(tile + off + (c & 7) * 16);
+        }
       }
+      // whatever lies in rows of V that are not live: 0 times it has to be 0
+      for (int r = valid + (lane >> 3); r < T; r += 4)
+#pragma unroll
+        for (int x = 0; x < G::V_BOXES; ++x) *reinterpret_cast<uint4*>(tile + 2 * G::K_BYTES + x * T * 128 + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+      __syncwarp();
     }
-    // scores: a lane's share of four rows of either branch, then sums over the lanes of a row; every exchange halves the values, so that
-    // each lane ends with the scores of NV rows of one branch (7 shuffles for 8 rows instead of 24 at D = 64)
-    float part[8];
-#pragma unroll
-    for (int br = 0; br < 2; ++br)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const uint4 w = *reinterpret_cast<const uint4*>(tile + br * G::K_BYTES + (r * 32 + lane) * 16);
-        f32x2 x = mul2(widen(unpack2<BF>(w.x)), q[br][0]);
-        x = fma2(widen(unpack2<BF>(w.y)), q[br][1], x);
-        x = fma2(widen(unpack2<BF>(w.z)), q[br][2], x);
-        x = fma2(widen(unpack2<BF>(w.w)), q[br][3], x);
-        float lo, hi;
-        up2(x, lo, hi);
-        part[br * 4 + r] = lo + hi;
-      }
-    float sc[NV];
-    {
-      float x[4], y[2];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) x[k] = (second ? part[4 + k] : part[k]) + __shfl_xor_sync(0xffffffffu, second ? part[k] : part[4 + k], M1);
-      const bool up = lane & M2;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) y[k] = (up ? x[2 + k] : x[k]) + __shfl_xor_sync(0xffffffffu, up ? x[k] : x[2 + k], M2);
-      if constexpr (NV == 2) {
-        sc[0] = y[0]; sc[1] = y[1];
-      } else {
-        const bool odd = lane & M3;
-        sc[0] = (odd ? y[1] : y[0]) + __shfl_xor_sync(0xffffffffu, odd ? y[0] : y[1], M3);
-        if constexpr (LPK == 16) sc[0] += __shfl_xor_sync(0xffffffffu, sc[0], 1);
-      }
-    }
-    int row[NV];
+    const uint32_t at_k = row_k + s * G::SLOT_BYTES, at_v = row_v + s * G::SLOT_BYTES;
+    float p[T / 16][2];
     float top = -INFINITY;
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int r = ((lane & M2) ? 2 : 0) + (NV == 2 ? v : (lane & M3) ? 1 : 0);
-      row[v] = r * (32 / LPK) + lane / LPK;
-      if (row[v] >= valid) sc[v] = -INFINITY;
-      top = fmaxf(top, sc[v]);
-    }
+    for (int g = 0; g < T / 16; ++g) {
+      float s1[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int x = 1; x < 32; x <<= 1)
-      if (x != M1 && !(LPK == 16 && x == 1)) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-    // the running maximum moves only when it is exceeded by more than 2^8: the probabilities stay far from fp32's limits either way
+      for (int k = 0; k < D / 16; ++k) {
+        const uint32_t off = (k >> 2) * T * G::K_ROW + g * 16 * G::K_ROW + (sw_k ^ ((k & 3) << 5));
+        uint32_t x[4];
+        ldsm4(x, at_k + off);
+        mma16816<BF>(s1, x, q[k][0], q[k][1]);
+        ldsm4(x, at_k + G::K_BYTES + off);
+        mma16816<BF>(s2, x, q[k][0], q[k][1]);
+      }
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        p[g][x] = (branch ? s2[2 * x] : s1[2 * x]) * a.scale_log2;
+        if (branch > 1 || g * 16 + x * 8 + (lane >> 2) >= valid) p[g][x] = -INFINITY;
+        if (TRACK && branch < 2) a.scores[((first + i) * 2 + branch) * T + g * 16 + x * 8 + (lane >> 2)] = p[g][x];
+        top = fmaxf(top, p[g][x]);
+      }
+    }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+    // the running maximum moves only when it is exceeded by more than 2^8: the probabilities stay inside fp16's range either way
     const bool need = top > m + 8.f;
     if (__any_sync(0xffffffffu, need)) {
       const float to = need ? top : m, f = ex2(m - to);
-      const float g = __shfl_xor_sync(0xffffffffu, f, M1);
-      const float f1 = second ? g : f, f2 = second ? f : g;
       l *= f;
       m = to;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        o[0][k] = mul2(o[0][k], pk2(f1, f1));
-        o[1][k] = mul2(o[1][k], pk2(f2, f2));
+      for (int k = 0; k < D / 8; ++k) {
+        o[k][0] *= f; o[k][1] *= f; o[k][2] *= f; o[k][3] *= f;
       }
     }
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const float p = ex2(sc[v] - m);
-      l += p;
-      prob[row[v] * 2 + (second ? 1 : 0)] = p;
-      if (TRACK && !(LPK == 16 && (lane & 1))) a.scores[((first + i) * 2 + (second ? 1 : 0)) * T + row[v]] = sc[v];
-    }
-    __syncwarp();
+    for (int g = 0; g < T / 16; ++g) {
+      uint32_t pb[2];
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {
-      const int vr = r * (32 / LPV) + lane / LPV;
-      uint4 w = *reinterpret_cast<const uint4*>(tile + 2 * G::K_BYTES + (r * 32 + lane) * 16);
-      if (valid < T && vr >= valid) w = make_uint4(0, 0, 0, 0);      // whatever lies there: 0 times it has to be 0
-      const float2 p = reinterpret_cast<const float2*>(prob)[vr];
-      const f32x2 p1 = pk2(p.x, p.x), p2 = pk2(p.y, p.y);
-      const f32x2 v0 = widen(unpack2<BF>(w.x)), v1 = widen(unpack2<BF>(w.y)), v2 = widen(unpack2<BF>(w.z)), v3 = widen(unpack2<BF>(w.w));
-      o[0][0] = fma2(v0, p1, o[0][0]); o[0][1] = fma2(v1, p1, o[0][1]); o[0][2] = fma2(v2, p1, o[0][2]); o[0][3] = fma2(v3, p1, o[0][3]);
-      o[1][0] = fma2(v0, p2, o[1][0]); o[1][1] = fma2(v1, p2, o[1][1]); o[1][2] = fma2(v2, p2, o[1][2]); o[1][3] = fma2(v3, p2, o[1][3]);
+      for (int x = 0; x < 2; ++x) {
+        const float e = ex2(p[g][x] - m);
+        l += e;
+        const float hi = to_float16b<BF>(from_float16b<BF>(e));
+        pb[x] = movmatrix(pack2<BF>(hi, e - hi));
+      }
+#pragma unroll
+      for (int k = 0; k < D / 8; ++k) {
+        uint32_t x[4];
+        ldsm4_trans(x, at_v + (k >> 2) * T * 128 + g * 16 * 128 + (sw_v ^ ((k & 3) << 5)));
+        mma16816<BF>(o[k], x, pb[0], pb[1]);
+      }
     }
+    if (valid < T) fence_proxy_async_smem();   // (rows were written by this warp)
     __syncwarp();                              // the tile is read: its slot takes the next one
     if (i + SLOTS < count) {
-      request(ahead, id, s, ahead.t == 0);
+      request(ahead, box, s, ahead.t == 0);
       if (i + SLOTS + 1 < count) {
         next(ahead);
-        id = page_ids(ahead);
+        box = look_up(ahead);
       }
     }
     if (cur.t == cur.n - 1 || i == count - 1) {
       // the stretch leaves this (sequence, head)
-      float ov[2][8];
-#pragma unroll
-      for (int br = 0; br < 2; ++br)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) up2(o[br][k], ov[br][2 * k], ov[br][2 * k + 1]);
-#pragma unroll
-      for (int x = LPV; x < 32; x <<= 1)
-#pragma unroll
-        for (int br = 0; br < 2; ++br)
-#pragma unroll
-          for (int k = 0; k < 8; ++k) ov[br][k] += __shfl_xor_sync(0xffffffffu, ov[br][k], x);
-      float ls = l;
-#pragma unroll
-      for (int x = 1; x < 32; x <<= 1)
-        if (x != M1 && !(LPK == 16 && x == 1)) ls += __shfl_xor_sync(0xffffffffu, ls, x);
-      const float mo = __shfl_xor_sync(0xffffffffu, m, M1), lo = __shfl_xor_sync(0xffffffffu, ls, M1);
+      l += __shfl_xor_sync(0xffffffffu, l, 4);
+      l += __shfl_xor_sync(0xffffffffu, l, 8);
+      l += __shfl_xor_sync(0xffffffffu, l, 16);
       const size_t at = size_t(worker) + size_t(cur.b) * a.c.h + cur.h;      // a piece's place: grows with every piece along the line
-      if (lane == 0) a.stats[at] = make_float4(m, ls, mo, lo);
-      if (lane < LPV) {
-        float4* to = a.acc + at * D + lane * 2;
+      if (lane < 2) reinterpret_cast<float2*>(a.stats + at)[lane] = make_float2(m, l);
+      if (branch < 2) {
+        float* to = reinterpret_cast<float*>(a.acc + at * D) + branch * 2 * D + (lane >> 2);
 #pragma unroll
-        for (int br = 0; br < 2; ++br) {
-          to[br * (D / 2)] = make_float4(ov[br][0], ov[br][1], ov[br][2], ov[br][3]);
-          to[br * (D / 2) + 1] = make_float4(ov[br][4], ov[br][5], ov[br][6], ov[br][7]);
+        for (int k = 0; k < D / 8; ++k) {
+          to[k * 16] = o[k][0] + o[k][1];
+          to[k * 16 + 8] = o[k][2] + o[k][3];
         }
       }
     }
@@ -536,9 +549,9 @@ __global__ void __launch_bounds__(JOIN_THREADS) diffattn_cache_join_kernel(const
       const float c1 = 1.f / j.l1, c2 = lam / j.l2;
       float* to = a.c.weights + (size_t)bh * a.c.slots;
       for (int e = lane; e < n * T; e += 32) {
-        int slot, in_page, valid;
+        int slot, valid;
         bool is_new;
-        attend_tile<T>(a, w.t + e / T, w.n, w.len, slot, in_page, valid, is_new);
+        attend_tile<T>(a, w.t + e / T, w.n, w.len, slot, valid, is_new);
         const int row = e % T;
         if (row >= valid || slot + row >= a.c.slots) continue;
         const float* s = a.scores + (u + e / T) * 2 * T + row;

@@ -3,29 +3,35 @@
 
 namespace {
 
-// How a tile of T rows is fetched.  A box has as many rows as a tile; where a page is smaller and divides a tile (and a box's rows fill
-// whole 128-byte lines of shared memory, which the engine asks for) a tile is put together from the boxes of several pages.
+// How a tile of T rows is fetched.  Where page size and tile have a common divisor of 8 or more (every page size that is a multiple of 8), tiles
+// run on over the pages in boxes of that many rows, each inside one page and, in shared memory, at a whole period of the swizzle.
+// Else a tile stays inside its page and its last one is not full (a page of 100 slots: 7 tiles of 16; a page of 1: a tile for every token).
 struct TileShape { int rows, box_rows, tiles_per_page; };
+int tile_rows(int D) { return D == 32 ? da::attend::Geo<32>::T : D == 64 ? da::attend::Geo<64>::T : da::attend::Geo<128>::T; }
 TileShape tile_shape(const DiffAttnCacheParams* p) {
-  const int T = 1024 / p->D;
-  if (p->page_size < T && T % p->page_size == 0 && p->page_size * p->D * 2 % 128 == 0) return {T, p->page_size, 1};
+  const int T = tile_rows(p->D);
+  int r = T;
+  while (p->page_size % r) r /= 2;             // (T is a power of two)
+  if (r >= 8) return {T, r, 0};
   return {T, T, (p->page_size + T - 1) / T};
 }
 // tiles of a full sequence
 long long most_tiles(const DiffAttnCacheParams* p) {
   const TileShape s = tile_shape(p);
   const long long slots = (long long)p->max_pages * p->page_size;
-  return (s.box_rows < s.rows ? (slots + s.rows - 1) / s.rows : (long long)p->max_pages * s.tiles_per_page) + 1;      // + 1: the new token
+  return (s.tiles_per_page ? (long long)p->max_pages * s.tiles_per_page : (slots + s.rows - 1) / s.rows) + 1;      // + 1: the new token
 }
 
-int attend_workers(int device) { return sm_count(device) * da::attend::WARPS; }
+int attend_workers(const DiffAttnCacheParams* p) {
+  return sm_count(p->device) * (p->D == 32 ? da::attend::Geo<32>::WARPS : p->D == 64 ? da::attend::Geo<64>::WARPS : da::attend::Geo<128>::WARPS);
+}
 
 struct AttendSpace {
   uint64_t prefix, length, position, stats, acc, scores, bytes;
 };
 AttendSpace attend_space(const DiffAttnCacheParams* p) {
   AttendSpace s;
-  const uint64_t pieces = uint64_t(attend_workers(p->device)) + uint64_t(p->B) * p->H;
+  const uint64_t pieces = uint64_t(attend_workers(p)) + uint64_t(p->B) * p->H;
   uint64_t at = 0;
   auto take = [&](uint64_t& where, uint64_t bytes) { where = at; at += round256(bytes); };
   take(s.prefix, 4 * (uint64_t(p->B) + 1));
@@ -33,7 +39,7 @@ AttendSpace attend_space(const DiffAttnCacheParams* p) {
   take(s.position, 4 * uint64_t(p->B));
   take(s.stats, 16 * pieces);
   take(s.acc, 16 * pieces * p->D);
-  take(s.scores, p->weights ? uint64_t(most_tiles(p)) * p->B * p->H * 2 * (1024 / p->D) * 4 : 0);
+  take(s.scores, p->weights ? uint64_t(most_tiles(p)) * p->B * p->H * 2 * tile_rows(p->D) * 4 : 0);
   s.bytes = at;
   return s;
 }
@@ -134,18 +140,18 @@ int attend_launch(const DiffAttnCacheParams* p, da::AttendArgs& a) {
   auto map = [&](CUtensorMap* m, const void* base, int width, int64_t page, int64_t head, int64_t slot, const char* what) {
     // (a dimension of one element needs a legal stride all the same)
     if (p->page_size == 1) slot = width;
-    return make_map<BF>(m, base, width, p->page_size, p->H, p->num_pages, slot, head, page, a.box_rows, what, width);
+    return make_map<BF>(m, base, width, p->page_size, p->H, p->num_pages, slot, head, page, a.box_rows, what, std::min(width, 64));
   };
   if ((rc = map(&k1, p->k1_pages, D, p->kp_stride_page, p->kp_stride_head, p->kp_stride_slot, "k1_pages"))) return rc;
   if ((rc = map(&k2, p->k2_pages, D, p->kp_stride_page, p->kp_stride_head, p->kp_stride_slot, "k2_pages"))) return rc;
   if ((rc = map(&v, p->v_pages, 2 * D, p->vp_stride_page, p->vp_stride_head, p->vp_stride_slot, "v_pages"))) return rc;
   auto kernel = da::diffattn_cache_attend_kernel<D, BF, TRACK>;
-  constexpr int most = da::attend::Geo<D>::SMEM + 4 * (da::attend::MAX_B + 1) + 128;
-  const int smem = da::attend::Geo<D>::SMEM + 4 * (p->B + 1) + 128;
+  constexpr int most = da::attend::Geo<D>::SMEM + 4 * da::attend::MAX_B;
+  const int smem = da::attend::Geo<D>::SMEM + 4 * p->B;
   if ((rc = set_smem(kernel, most, p->device))) return rc;
   const cudaStream_t stream = static_cast<cudaStream_t>(p->stream);
   const int sms = sm_count(p->device);
-  if ((rc = launch(kernel, dim3(sms), da::attend::THREADS, smem, stream, false, k1, k2, v, a))) return rc;
+  if ((rc = launch(kernel, dim3(sms), da::attend::Geo<D>::THREADS, smem, stream, false, k1, k2, v, a))) return rc;
   const int grid = TRACK ? sms * 4 : std::min(p->B * p->H, sms * 8);
   return launch(da::diffattn_cache_join_kernel<D, BF, TRACK>, dim3(grid), da::JOIN_THREADS, 0, stream, true, a);
 }
@@ -234,7 +240,8 @@ int diffattn_cache_attend(const DiffAttnCacheParams* p) {
   a.gain = p->gain; a.y = static_cast<__half*>(p->y);
   const TileShape shape = tile_shape(p);
   a.box_rows = shape.box_rows; a.tiles_per_page = shape.tiles_per_page;
-  a.workers = attend_workers(p->device);
+  a.tiles_magic = shape.tiles_per_page > 1 ? uint32_t(((1ull << 32) + shape.tiles_per_page - 1) / shape.tiles_per_page) : 0u;
+  a.workers = attend_workers(p);
   uint8_t* ws = static_cast<uint8_t*>(p->workspace);
   a.prefix = reinterpret_cast<int*>(ws + space.prefix);
   a.length = reinterpret_cast<int*>(ws + space.length);

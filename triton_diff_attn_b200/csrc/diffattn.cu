@@ -86,10 +86,10 @@ PFN_cuTensorMapEncodeTiled_v12000 get_encode() {
 struct MapKey {
   const void* base;
   int64_t s_row, s2, s3;
-  int32_t cols, rows, d2, d3, box_rows, bf, plain_cols;
+  int32_t cols, rows, d2, d3, box_rows, bf, box_cols;
   bool operator==(const MapKey& o) const {
     return base == o.base && s_row == o.s_row && s2 == o.s2 && s3 == o.s3 && cols == o.cols && rows == o.rows && d2 == o.d2 &&
-           d3 == o.d3 && box_rows == o.box_rows && bf == o.bf && plain_cols == o.plain_cols;
+           d3 == o.d3 && box_rows == o.box_rows && bf == o.bf && box_cols == o.box_cols;
   }
 };
 struct MapKeyHash {
@@ -99,7 +99,7 @@ struct MapKeyHash {
     mix(uint64_t(k.s_row)); mix(uint64_t(k.s2)); mix(uint64_t(k.s3));
     mix((uint64_t(uint32_t(k.cols)) << 32) | uint32_t(k.rows));
     mix((uint64_t(uint32_t(k.d2)) << 32) | uint32_t(k.d3));
-    mix((uint64_t(uint32_t(k.box_rows)) << 1) | uint32_t(k.bf) | (uint64_t(uint32_t(k.plain_cols)) << 32));
+    mix((uint64_t(uint32_t(k.box_rows)) << 1) | uint32_t(k.bf) | (uint64_t(uint32_t(k.box_cols)) << 32));
     return size_t(h);
   }
 };
@@ -110,12 +110,12 @@ thread_local std::unordered_map<const void*, int> g_ptr_device;         // base 
 thread_local int g_sm_count[kMaxDevices] = {0};
 
 // 16-bit (fp16, or bf16 when BF) tensor [d3, d2, rows, cols] with element strides (s3, s2, s_row, 1); box = box_rows x 64 columns,
-// 128-byte swizzle (the layout the tcgen05 shared-memory descriptors in sm100.cuh describe).  plain_cols > 0: box = box_rows x plain_cols, rows
-// one behind the other without a swizzle.
+// 128-byte swizzle (the layout the tcgen05 shared-memory descriptors in sm100.cuh describe).  box_cols 32: boxes of
+// 32 columns, 64-byte swizzle (64-byte rows read as matrices by mma.sync).
 template <bool BF>
 int make_map(CUtensorMap* map, const void* base, int cols, int rows, int d2, int d3, int64_t s_row, int64_t s2, int64_t s3,
-             int box_rows, const char* what, int plain_cols = 0) {
-  const MapKey key{base, s_row, s2, s3, cols, rows, d2, d3, box_rows, BF ? 1 : 0, plain_cols};
+             int box_rows, const char* what, int box_cols = 64) {
+  const MapKey key{base, s_row, s2, s3, cols, rows, d2, d3, box_rows, BF ? 1 : 0, box_cols};
   {
     auto it = g_maps.find(key);
     if (it != g_maps.end()) {
@@ -130,11 +130,11 @@ int make_map(CUtensorMap* map, const void* base, int cols, int rows, int d2, int
   // a size-1 dimension's stride is never used, but the encoder still wants a legal value
   if (d2 == 1) strides[1] = strides[0] * cuuint64_t(rows);
   if (d3 == 1) strides[2] = strides[1] * cuuint64_t(d2);
-  // The box is always 64 columns (128 bytes, one swizzle row).  A tensor narrower than that (head dim 32)
+  // A box of 64 columns is 128 bytes, one swizzle row.  A tensor narrower than that (head dim 32)
   // is padded by the TMA engine: out-of-range elements arrive as zeros.
-  cuuint32_t box[4] = {plain_cols ? cuuint32_t(plain_cols) : 64u, cuuint32_t(box_rows), 1, 1};
+  cuuint32_t box[4] = {cuuint32_t(box_cols), cuuint32_t(box_rows), 1, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
-  const CUtensorMapSwizzle sw = plain_cols ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B;
+  const CUtensorMapSwizzle sw = box_cols == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
   CUresult r = enc(map, BF ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
                    CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
