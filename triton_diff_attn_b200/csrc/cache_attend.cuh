@@ -49,7 +49,7 @@ template <int D>
 struct Geo {
   static constexpr int T = D == 32 ? 32 : 16;  // tokens per tile: 8 KB of K1, K2, V (D = 128: 16 KB)
   static constexpr int WARPS = D == 128 ? 4 : 8, THREADS = WARPS * 32;
-  static constexpr int SLOTS = 3;              // tiles in flight per warp: 192 KB of requests per SM
+  static constexpr int SLOTS = 2;              // tiles in flight per warp
   // a tile in shared memory: boxes of T rows of 128 bytes (K at D = 32: 64 bytes), swizzled by the engine: K1, K2, V
   static constexpr int K_ROW = D == 32 ? 64 : 128, K_BOXES = D == 128 ? 2 : 1, V_BOXES = D / 32;
   static constexpr int K_BYTES = T * D * 2, V_BYTES = 2 * K_BYTES, SLOT_BYTES = 2 * K_BYTES + V_BYTES;
@@ -457,39 +457,66 @@ __device__ __forceinline__ Joined join_stats(const float4* stats, int w0, int w1
   return j;
 }
 
-constexpr int JOIN_THREADS = 256;
+// Many threads where a (sequence, head) has many pieces (few of them share the workers): what counts is the chain of loads, prefix, statistics,
+// sums, each about 0.7 us away in L2, so all of a thread's loads go out together and there are enough threads to need one round of them.
+constexpr int JOIN_AHEAD = 4;                  // pieces whose sums a thread requests before it knows their weights
 
-template <int D, bool BF, bool TRACK>
-__global__ void __launch_bounds__(JOIN_THREADS) diffattn_cache_join_kernel(const __grid_constant__ AttendArgs a) {
+template <int D, int JT, bool BF, bool TRACK>
+__global__ void __launch_bounds__(JT) diffattn_cache_join_kernel(const __grid_constant__ AttendArgs a) {
   constexpr int T = attend::Geo<D>::T;
-  constexpr int GROUPS = JOIN_THREADS / D;     // pieces summed side by side: a thread has four of a piece's 4 D sums
-  __shared__ float4 red[JOIN_THREADS];
+  constexpr int GROUPS = JT / D;               // pieces summed side by side: a thread has four of a piece's 4 D sums
+  __shared__ float4 red[JT];
   __shared__ float ssq[2 * D / 32];
+  extern __shared__ int line[];                // with weights: prefix sums and lengths (a search in global memory is a chain of loads)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   griddep_wait();
   const int nb = a.c.b, heads = a.c.h;
+  if constexpr (TRACK) {
+    for (int b = threadIdx.x; b <= nb; b += JT) {
+      line[b] = a.prefix[b];
+      if (b < nb) line[nb + 1 + b] = a.length[b];
+    }
+    __syncthreads();
+  }
   const long long units = (long long)a.prefix[nb] * heads;
   const int workers = int(min((long long)a.workers, units));
   const float lam = load_lambda(a.lambda_ptr, a.lambda_dtype);
   for (int bh = blockIdx.x; bh < nb * heads; bh += gridDim.x) {
     const int b = bh / heads, head = bh - b * heads;
     const int n = a.prefix[b + 1] - a.prefix[b];
+    const float gain = a.gain && threadIdx.x < 2 * D ? a.gain[threadIdx.x] : 1.f;
     float out = 0.f;
     if (n > 0) {
       int w0, w1;
       piece_range(units, workers, (long long)a.prefix[b] * heads + (long long)head * n, n, w0, w1);
       const float4* stats = a.stats + bh;
-      const Joined j = join_stats(stats, w0, w1, lane);
       const int col = threadIdx.x % D, group = threadIdx.x / D;
       const bool second = col >= D / 2;
+      const float4* acc = a.acc + (size_t)bh * D + col;
+      float4 x[JOIN_AHEAD];
+      float mx[JOIN_AHEAD];
+#pragma unroll
+      for (int k = 0; k < JOIN_AHEAD; ++k) {
+        const int w = w0 + group + k * GROUPS;
+        mx[k] = -INFINITY;
+        x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (w <= w1) {
+          x[k] = acc[(size_t)w * D];
+          mx[k] = second ? stats[w].z : stats[w].x;
+        }
+      }
+      const Joined j = join_stats(stats, w0, w1, lane);
       const float top = second ? j.m2 : j.m1;
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+      auto add = [&](const float4& v, float m) {
+        const float c = ex2(m - top);
+        sum.x += c * v.x; sum.y += c * v.y; sum.z += c * v.z; sum.w += c * v.w;
+      };
+#pragma unroll
+      for (int k = 0; k < JOIN_AHEAD; ++k)
+        if (w0 + group + k * GROUPS <= w1) add(x[k], mx[k]);
 #pragma unroll 4
-      for (int w = w0 + group; w <= w1; w += GROUPS) {
-        const float4 x = a.acc[(size_t(bh) + w) * D + col];
-        const float c = ex2((second ? stats[w].z : stats[w].x) - top);
-        sum.x += c * x.x; sum.y += c * x.y; sum.z += c * x.z; sum.w += c * x.w;
-      }
+      for (int w = w0 + group + JOIN_AHEAD * GROUPS; w <= w1; w += GROUPS) add(acc[(size_t)w * D], second ? stats[w].z : stats[w].x);
       red[threadIdx.x] = sum;
       __syncthreads();
       if (threadIdx.x < 2 * D) {
@@ -514,10 +541,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) diffattn_cache_join_kernel(const
         out *= rsqrtf(sq / float(2 * D) + a.eps) * a.out_scale;
       }
     }
-    if (threadIdx.x < 2 * D) {
-      if (a.gain) out *= a.gain[threadIdx.x];
-      a.y[size_t(bh) * 2 * D + threadIdx.x] = from_float16b<BF>(out);
-    }
+    if (threadIdx.x < 2 * D) a.y[size_t(bh) * 2 * D + threadIdx.x] = from_float16b<BF>(out * gain);
     if (a.nk1 && threadIdx.x == 0) {
       const int len = a.length[b];
       if (len < a.c.slots) {
@@ -534,33 +558,51 @@ __global__ void __launch_bounds__(JOIN_THREADS) diffattn_cache_join_kernel(const
   }
   if constexpr (TRACK) {
     // the same line of tiles, cut into the warps of this grid
-    const int takers = int(min((long long)gridDim.x * (JOIN_THREADS / 32), units));
+    const int takers = int(min((long long)gridDim.x * (JT / 32), units));
     const int taker = warp * int(gridDim.x) + int(blockIdx.x);
     if (taker >= takers) return;
     long long u = stretch_begin(units, takers, taker);
     const long long end = stretch_begin(units, takers, taker + 1);
-    TileWalk w = walk_at(a, a.prefix, a.length, u);
+    TileWalk w = walk_at(a, line, line + nb + 1, u);
     while (u < end) {
       const int n = int(min((long long)(w.n - w.t), end - u));      // tiles of this (sequence, head)
       const int bh = w.b * heads + w.h;
       int w0, w1;
       piece_range(units, workers, u - w.t, w.n, w0, w1);
-      const Joined j = join_stats(a.stats + bh, w0, w1, lane);
-      const float c1 = 1.f / j.l1, c2 = lam / j.l2;
       float* to = a.c.weights + (size_t)bh * a.c.slots;
-      for (int e = lane; e < n * T; e += 32) {
-        int slot, valid;
-        bool is_new;
-        attend_tile<T>(a, w.t + e / T, w.n, w.len, slot, valid, is_new);
-        const int row = e % T;
-        if (row >= valid || slot + row >= a.c.slots) continue;
-        const float* s = a.scores + (u + e / T) * 2 * T + row;
-        const float x = fabsf(ex2(s[0] - j.m1) * c1 - ex2(s[T] - j.m2) * c2);
-        to[slot + row] = is_new ? x : to[slot + row] + x;
+      constexpr int ROUND = 4;                 // tokens of a lane whose loads are under way together
+      Joined j;
+      float c1 = 0.f, c2 = 0.f;
+      for (int e0 = 0; e0 < n * T; e0 += 32 * ROUND) {      // (all lanes: they join the statistics together)
+        float s1[ROUND], s2[ROUND], old[ROUND];
+        int at[ROUND];                         // -1: no token
+#pragma unroll
+        for (int k = 0; k < ROUND; ++k) {
+          const int e = e0 + lane + 32 * k, row = e % T;
+          at[k] = -1;
+          if (e >= n * T) continue;
+          int slot, valid;
+          bool is_new;
+          attend_tile<T>(a, w.t + e / T, w.n, w.len, slot, valid, is_new);
+          if (row >= valid || slot + row >= a.c.slots) continue;
+          at[k] = slot + row;
+          const float* s = a.scores + (u + e / T) * 2 * T + row;
+          s1[k] = s[0];
+          s2[k] = s[T];
+          old[k] = is_new ? 0.f : to[at[k]];
+        }
+        if (e0 == 0) {
+          j = join_stats(a.stats + bh, w0, w1, lane);
+          c1 = 1.f / j.l1;
+          c2 = lam / j.l2;
+        }
+#pragma unroll
+        for (int k = 0; k < ROUND; ++k)
+          if (at[k] >= 0) to[at[k]] = old[k] + fabsf(ex2(s1[k] - j.m1) * c1 - ex2(s2[k] - j.m2) * c2);
       }
       u += n;
       w.t += n - 1;
-      if (u < end) walk_next(a, a.prefix, a.length, w);
+      if (u < end) walk_next(a, line, line + nb + 1, w);
     }
   }
 }

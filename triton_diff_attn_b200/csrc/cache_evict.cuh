@@ -5,8 +5,9 @@
 // that the others leave below it, the k-th survivor into the k-th hole.  Sources and destinations never overlap, every move is independent of
 // the others, and a call that evicts a few tokens moves a few rows.
 //
-// Two kernels: the selection (a CTA per (sequence, head): 8 bytes per token read, the rest in shared memory) writes a list of moves, the
-// second one carries them out, spread over all SMs whatever the number of heads is.
+// The selection takes a CTA per (sequence, head): 8 bytes per token read, the rest in shared memory.  Where its moves are few, or the CTAs enough
+// to fill the GPU, it carries them out too; else it writes them down for a second kernel that spreads them over all SMs.  Either way the
+// lengths change in a kernel behind it, when every head has read them.
 #pragma once
 #include "cache.cuh"
 
@@ -19,6 +20,7 @@ struct EvictArgs {
   int* count;                        // [b * h] moves
   int2* moves;                       // [b * h][most] {from, to}
   int cached_keys;                   // the selection keeps all keys in shared memory
+  int moves_at_once;                 // the selection carries its moves out
 };
 
 constexpr int SELECT_THREADS = 512, SELECT_WARPS = SELECT_THREADS / 32;
@@ -27,14 +29,14 @@ constexpr int SELECT_MOST_KEYS = 48 * 1024;      // that fit in shared memory
 // Order of a slot: whole numbers, larger = rather kept.  NaN counts as larger than every number, -0 as 0.
 __device__ __forceinline__ uint32_t evict_key(const EvictArgs& a, long long at, int newest_from) {
   const int pos = a.c.positions[at];
+  const float w = a.c.weights ? a.c.weights[at] : 0.f;
   if (pos >= newest_from) return 0xffffffffu;
   if (!a.c.weights) return uint32_t(max(pos, 0));
-  const float w = a.c.weights[at];
   const uint32_t u = w != w ? 0x7fc00000u : __float_as_uint(w + 0.f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// sum of `x` over the threads before this one; `total`: over all.  `buf`: SELECT_WARPS ints, free again after the call's second barrier
+// sum of `x` over the threads before this one; `total`: over all.  `buf`: SELECT_WARPS ints of this call's own
 __device__ __forceinline__ int block_before(int x, int* buf, int& total) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int incl = x;
@@ -53,110 +55,167 @@ __device__ __forceinline__ int block_before(int x, int* buf, int& total) {
   }
   total = __shfl_sync(0xffffffffu, s, 31);
   const int before = __shfl_sync(0xffffffffu, s, max(warp - 1, 0));
-  __syncthreads();
   return (warp ? before : 0) + incl - x;
 }
 
+// Rows first, first + step, ... of a list of moves, UNROLL of them under way together.  Thread: one 16-byte piece of a row.
+template <int D, int THREADS, int UNROLL>
+__device__ __forceinline__ void move_rows(const EvictArgs& a, int bh, const int2* list, int count, int block, int blocks) {
+  constexpr int PARTS = D / 2, ROWS = THREADS / PARTS;
+  const CacheArgs& c = a.c;
+  const int b = bh / c.h, head = bh - b * c.h, part = threadIdx.x % PARTS;
+  for (int r0 = block * (ROWS * UNROLL) + threadIdx.x / PARTS; r0 < count; r0 += blocks * (ROWS * UNROLL)) {
+    uint4 x[UNROLL];
+    uint4* to[UNROLL];
+    int2 mv[UNROLL];
+#pragma unroll
+    for (int i = 0; i < UNROLL; ++i) mv[i] = r0 + i * ROWS < count ? list[r0 + i * ROWS] : make_int2(-1, -1);
+#pragma unroll
+    for (int i = 0; i < UNROLL; ++i) {
+      to[i] = nullptr;
+      if (mv[i].x < 0) continue;
+      const int pf = cache_page(c, mv[i].x), pt = cache_page(c, mv[i].y);
+      const int from = cache_page_id(c, b, pf), dest = cache_page_id(c, b, pt);
+      if (from < 0 || dest < 0) continue;
+      x[i] = *cache_piece<D>(c, from, head, mv[i].x - pf * c.page_size, part);
+      to[i] = cache_piece<D>(c, dest, head, mv[i].y - pt * c.page_size, part);
+    }
+#pragma unroll
+    for (int i = 0; i < UNROLL; ++i) {
+      if (to[i]) *to[i] = x[i];
+      if (mv[i].x >= 0 && part == 0) {
+        const long long base = (long long)bh * c.slots;
+        c.positions[base + mv[i].y] = c.positions[base + mv[i].x];
+        if (c.weights) c.weights[base + mv[i].y] = c.weights[base + mv[i].x];
+      }
+    }
+  }
+}
+
+constexpr int SELECT_LIST = 512;                 // moves that the selection keeps in shared memory
+
+template <int D>
 __global__ void __launch_bounds__(SELECT_THREADS) diffattn_cache_select_kernel(const EvictArgs a) {
   extern __shared__ uint32_t keys[];
-  __shared__ int hist[256], buf[SELECT_WARPS], found[2];
+  __shared__ int hist[4][256], buf[2][SELECT_WARPS];
+  __shared__ int2 near_list[SELECT_LIST];
   const CacheArgs& c = a.c;
   griddep_launch();
-  const int bh = blockIdx.x, b = bh / c.h, tid = threadIdx.x;
+  const int bh = blockIdx.x, b = bh / c.h, tid = threadIdx.x, lane = tid & 31;
+  const int newest_from = c.next_position[b] - a.recent;
   const int len = cache_length(c, b);
   if (len <= a.keep) {
     if (tid == 0) a.count[bh] = 0;
     return;
   }
+  for (int i = tid; i < 4 * 256; i += SELECT_THREADS) hist[0][i] = 0;
+  __syncthreads();
   const long long base = (long long)bh * c.slots;
-  const int newest_from = c.next_position[b] - a.recent;
-  if (a.cached_keys)
-    for (int i = tid; i < len; i += SELECT_THREADS) keys[i] = evict_key(a, base + i, newest_from);
-  auto key = [&](int i) { return a.cached_keys ? keys[i] : evict_key(a, base + i, newest_from); };      // (each thread reads its own)
   // the keep-th largest key, eight bits at a time: how many keys that agree with the bits so far have each next digit
+  auto key = [&](int i) { return a.cached_keys ? keys[i] : evict_key(a, base + i, newest_from); };
+#pragma unroll 4
+  for (int i = tid; i < len; i += SELECT_THREADS) {
+    const uint32_t k = evict_key(a, base + i, newest_from);
+    if (a.cached_keys) keys[i] = k;
+    atomicAdd(&hist[0][k >> 24], 1);
+  }
   uint32_t prefix = 0;
-  int want = a.keep;                 // of the keys that agree with `prefix`, this many stay
+  int want = a.keep, alike = 0;      // of the `alike` keys that agree with `prefix`, `want` stay
 #pragma unroll 1
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += SELECT_THREADS) hist[i] = 0;
-    __syncthreads();
-    for (int i = tid; i < len; i += SELECT_THREADS) {
-      const uint32_t k = key(i);
-      if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255], 1);
+  for (int digit = 0; digit < 4; ++digit) {
+    const int shift = 24 - 8 * digit;
+    if (digit > 0) {
+      for (int i = tid; i < len; i += SELECT_THREADS) {
+        const uint32_t k = key(i);
+        if (k >> (shift + 8) == prefix >> (shift + 8)) atomicAdd(&hist[digit][(k >> shift) & 255], 1);
+      }
     }
     __syncthreads();
-    // digits from the largest down: thread t has digit 255 - t
-    const int mine = tid < 256 ? hist[255 - tid] : 0;
-    int total;
-    const int above = block_before(mine, buf, total);
-    if (mine && above < want && above + mine >= want) {
-      found[0] = 255 - tid;
-      found[1] = above;
+    // every warp by itself: lane l has digits 255 - 8 l down to 248 - 8 l
+    int n[8], sum = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum += n[k] = hist[digit][255 - 8 * lane - k];
+    int above = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, above, o);
+      if (lane >= o) above += y;
     }
-    __syncthreads();
-    prefix |= uint32_t(found[0]) << shift;
-    want -= found[1];
+    const int owner = __ffs(__ballot_sync(0xffffffffu, above >= want)) - 1;      // the lane whose digits hold the want-th key
+    above -= sum;
+    int d = 0, left = 0, size = 0;
+    bool found = false;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (!found && above + n[k] >= want) {
+        found = true;
+        d = 255 - 8 * lane - k; left = want - above; size = n[k];
+      }
+      above += n[k];
+    }
+    prefix |= uint32_t(__shfl_sync(0xffffffffu, d, owner)) << shift;
+    want = __shfl_sync(0xffffffffu, left, owner);
+    alike = __shfl_sync(0xffffffffu, size, owner);
+    if (alike == want) break;        // all of them stay: whatever their lower bits are
   }
-  // keys above `prefix` stay, and the first `want` of those equal to it; survivors behind `keep` and holes below it in slot order
-  int equal = 0, survivors = 0, holes = 0;
-  for (int i0 = 0; i0 < len; i0 += SELECT_THREADS) {
-    const int i = i0 + tid;
-    const uint32_t k = i < len ? key(i) : 0;
-    const bool eq = i < len && k == prefix;
-    int total;
-    const int rank = equal + block_before(eq, buf, total);
-    equal += total;
-    const bool kept = i < len && (k > prefix || (eq && rank < want));
-    const bool moves = kept && i >= a.keep, hole = i < a.keep && !kept;
-    const int at = block_before((moves ? 1 : 0) | (hole ? 0x10000 : 0), buf, total);      // both counts at once: at most SELECT_THREADS each
-    int2* list = a.moves + (long long)bh * a.most;
-    if (moves) list[survivors + (at & 0xffff)].x = i;
-    if (hole) list[holes + (at >> 16)].y = i;
-    survivors += total & 0xffff;
-    holes += total >> 16;
+  // Keys above `prefix` stay, and of those that agree with it the first `want`.  Survivors behind `keep` and holes below it in slot order: a
+  // thread has a run of slots (an odd number, so that a warp's reads fall into different banks)
+  const int run = ((len + SELECT_THREADS - 1) / SELECT_THREADS) | 1;
+  const int i0 = min(tid * run, len), i1 = min(i0 + run, len);
+  int rank = 0, total;
+  if (alike != want) {               // (all 32 bits of `prefix` are known)
+    int n = 0;
+    for (int i = i0; i < i1; ++i) n += key(i) == prefix;
+    rank = block_before(n, buf[0], total);
   }
-  if (tid == 0) a.count[bh] = survivors;
+  auto stays = [&](uint32_t k, int& r) {
+    if (alike == want) return k >= prefix;
+    if (k != prefix) return k > prefix;
+    return r++ < want;
+  };
+  int moves = 0, holes = 0, r = rank;
+  for (int i = i0; i < i1; ++i) {
+    const bool kept = stays(key(i), r);
+    moves += kept && i >= a.keep;
+    holes += !kept && i < a.keep;
+  }
+  int2* list = a.most <= SELECT_LIST ? near_list : a.moves + (long long)bh * a.most;
+  const int holes_before = block_before(holes, buf[1], total);
+  __syncthreads();
+  int at = block_before(moves, buf[1], total);
+  int to = holes_before;
+  r = rank;
+  for (int i = i0; i < i1; ++i) {
+    const bool kept = stays(key(i), r);
+    if (kept && i >= a.keep) list[at++].x = i;
+    if (!kept && i < a.keep) list[to++].y = i;
+  }
+  __syncthreads();
+  if (a.moves_at_once) {
+    move_rows<D, SELECT_THREADS, 4>(a, bh, list, total, 0, 1);
+    total = 0;
+  } else if (list == near_list) {
+    for (int i = tid; i < total; i += SELECT_THREADS) a.moves[(long long)bh * a.most + i] = list[i];
+  }
+  if (tid == 0) a.count[bh] = total;
 }
 
-constexpr int MOVE_THREADS = 256, MOVE_UNROLL = 2;
+constexpr int MOVE_THREADS = 256, MOVE_UNROLL = 4;
 
+// Grid (wide, b * h): the moves that the selection wrote down.
 template <int D>
 __global__ void __launch_bounds__(MOVE_THREADS) diffattn_cache_move_kernel(const EvictArgs a) {
-  constexpr int PARTS = D / 2, ROWS = MOVE_THREADS / PARTS;
-  const CacheArgs& c = a.c;
   griddep_wait();
-  const int part = threadIdx.x % PARTS;
-  for (int bh = blockIdx.y; bh < c.b * c.h; bh += gridDim.y) {
-    const int b = bh / c.h, head = bh - b * c.h, count = a.count[bh];
-    const int2* list = a.moves + (long long)bh * a.most;
-    for (int r0 = blockIdx.x * (ROWS * MOVE_UNROLL) + threadIdx.x / PARTS; r0 < count; r0 += gridDim.x * (ROWS * MOVE_UNROLL)) {
-      uint4 x[MOVE_UNROLL];
-      int2 mv[MOVE_UNROLL];
-      bool ok[MOVE_UNROLL];
-#pragma unroll
-      for (int i = 0; i < MOVE_UNROLL; ++i) {
-        const int r = r0 + i * ROWS;
-        ok[i] = r < count;
-        if (!ok[i]) continue;
-        mv[i] = list[r];
-        const int p = cache_page(c, mv[i].x), page = cache_page_id(c, b, p);
-        ok[i] = page >= 0;
-        if (ok[i]) x[i] = *cache_piece<D>(c, page, head, mv[i].x - p * c.page_size, part);
-      }
-#pragma unroll
-      for (int i = 0; i < MOVE_UNROLL; ++i) {
-        if (!ok[i]) continue;
-        const int p = cache_page(c, mv[i].y), page = cache_page_id(c, b, p);
-        if (page >= 0) *cache_piece<D>(c, page, head, mv[i].y - p * c.page_size, part) = x[i];
-        if (part == 0) {
-          const long long base = (long long)bh * c.slots;
-          c.positions[base + mv[i].y] = c.positions[base + mv[i].x];
-          if (c.weights) c.weights[base + mv[i].y] = c.weights[base + mv[i].x];
-        }
-      }
-    }
-    if (blockIdx.x == 0 && head == 0 && threadIdx.x == 0 && c.lengths[b] > a.keep) c.lengths[b] = a.keep;
-  }
+  const int bh = blockIdx.y, b = bh / a.c.h;
+  move_rows<D, MOVE_THREADS, MOVE_UNROLL>(a, bh, a.moves + (long long)bh * a.most, a.count[bh], blockIdx.x, gridDim.x);
+  if (blockIdx.x == 0 && bh == b * a.c.h && threadIdx.x == 0 && a.c.lengths[b] > a.keep) a.c.lengths[b] = a.keep;
+}
+
+// The lengths alone, where the selection has moved everything.
+__global__ void __launch_bounds__(MOVE_THREADS) diffattn_cache_shorten_kernel(const EvictArgs a) {
+  griddep_wait();
+  const int b = blockIdx.x * MOVE_THREADS + threadIdx.x;
+  if (b < a.c.b && a.c.lengths[b] > a.keep) a.c.lengths[b] = a.keep;
 }
 
 }  // namespace da

@@ -152,14 +152,35 @@ int attend_launch(const DiffAttnCacheParams* p, da::AttendArgs& a) {
   const cudaStream_t stream = static_cast<cudaStream_t>(p->stream);
   const int sms = sm_count(p->device);
   if ((rc = launch(kernel, dim3(sms), da::attend::Geo<D>::THREADS, smem, stream, false, k1, k2, v, a))) return rc;
-  const int grid = TRACK ? sms * 4 : std::min(p->B * p->H, sms * 8);
-  return launch(da::diffattn_cache_join_kernel<D, BF, TRACK>, dim3(grid), da::JOIN_THREADS, 0, stream, true, a);
+  // 1024 threads for more than a dozen pieces a (sequence, head): B1 H16 N16384 D64 (74 pieces) XX us instead of XX
+  const int bh = p->B * p->H, line = TRACK ? 4 * (2 * p->B + 1) : 0;
+  if (a.workers > 12 * bh) {
+    const int grid = TRACK ? sms * 2 : std::min(bh, sms * 2);
+    return launch(da::diffattn_cache_join_kernel<D, 1024, BF, TRACK>, dim3(grid), 1024, line, stream, true, a);
+  }
+  const int grid = TRACK ? sms * 4 : std::min(bh, sms * 8);
+  return launch(da::diffattn_cache_join_kernel<D, 256, BF, TRACK>, dim3(grid), 256, line, stream, true, a);
 }
 template <int D>
 int attend_launch(const DiffAttnCacheParams* p, da::AttendArgs& a) {
   const bool bf = p->io_dtype == DIFFATTN_IO_BF16;
   if (p->weights) return bf ? attend_launch<D, true, true>(p, a) : attend_launch<D, false, true>(p, a);
   return bf ? attend_launch<D, true, false>(p, a) : attend_launch<D, false, false>(p, a);
+}
+
+template <int D>
+int evict_launch(const DiffAttnCacheParams* p, const da::EvictArgs& a) {
+  int rc;
+  const cudaStream_t stream = static_cast<cudaStream_t>(p->stream);
+  const int bh = p->B * p->H;
+  if ((rc = set_smem(da::diffattn_cache_select_kernel<D>, da::SELECT_MOST_KEYS * 4, p->device))) return rc;
+  if ((rc = launch(da::diffattn_cache_select_kernel<D>, dim3(bh), da::SELECT_THREADS, a.cached_keys ? a.c.slots * 4 : 0, stream, false, a))) return rc;
+  if (a.moves_at_once)
+    return launch(da::diffattn_cache_shorten_kernel, dim3((p->B + da::MOVE_THREADS - 1) / da::MOVE_THREADS), da::MOVE_THREADS, 0, stream, true, a);
+  // as many CTAs as the SMs hold, spread over the (sequence, head)s, but no more than there can be moves for
+  const int rows = da::MOVE_THREADS / (D / 2) * da::MOVE_UNROLL;
+  const int wide = std::max(1, std::min((a.most + rows - 1) / rows, (sm_count(p->device) * 8 + bh - 1) / bh));
+  return launch(da::diffattn_cache_move_kernel<D>, dim3(wide, bh), da::MOVE_THREADS, 0, stream, true, a);
 }
 
 }  // namespace
@@ -271,14 +292,9 @@ int diffattn_cache_evict(const DiffAttnCacheParams* p) {
   a.count = static_cast<int*>(p->workspace);
   a.moves = reinterpret_cast<int2*>(static_cast<uint8_t*>(p->workspace) + round256(4 * uint64_t(bh)));
   a.cached_keys = a.c.slots <= da::SELECT_MOST_KEYS ? 1 : 0;
-  const cudaStream_t stream = static_cast<cudaStream_t>(p->stream);
-  if ((rc = set_smem(da::diffattn_cache_select_kernel, da::SELECT_MOST_KEYS * 4, p->device))) return rc;
-  if ((rc = launch(da::diffattn_cache_select_kernel, dim3(bh), da::SELECT_THREADS, a.cached_keys ? a.c.slots * 4 : 0, stream, false, a))) return rc;
-  // as many CTAs as the SMs hold, spread over the (sequence, head)s, but no more than there can be moves for
-  const int rows = da::MOVE_THREADS / (p->D / 2) * da::MOVE_UNROLL;
-  const int wide = std::max(1, std::min((a.most + rows - 1) / rows, (sm_count(p->device) * 8 + bh - 1) / bh));
-  auto kernel = p->D == 32 ? da::diffattn_cache_move_kernel<32> : p->D == 64 ? da::diffattn_cache_move_kernel<64> : da::diffattn_cache_move_kernel<128>;
-  return launch(kernel, dim3(wide, bh), da::MOVE_THREADS, 0, stream, true, a);
+  const int sms = sm_count(p->device);
+  a.moves_at_once = a.most <= 64 || bh >= sms ? 1 : 0;
+  return p->D == 32 ? evict_launch<32>(p, a) : p->D == 64 ? evict_launch<64>(p, a) : evict_launch<128>(p, a);
 }
 
 }  // extern "C"
