@@ -190,9 +190,7 @@ class DiffAttnCache:
 
     def reset(self) -> None:
         """Every sequence starts anew: nothing is cached."""
-        self._lengths.zero_()
-        if self._next_position is not None:
-            self._next_position.zero_()
+        torch._foreach_zero_([t for t in (self._lengths, self._next_position) if t is not None])      # one launch
 
     def append(self, k1, k2, v, counts=None) -> None:
         """Stores the tokens k1, k2 [B, H, T, D], v [B, H, T, 2D] behind each sequence's last one.  `counts` (an integer tensor [B]): sequence b

@@ -75,19 +75,49 @@ struct CacheAppendArgs {
 
 __device__ __forceinline__ int append_count(const CacheAppendArgs& a, int b) { return a.counts ? min(max(a.counts[b], 0), a.t) : a.t; }
 
+// Where the rows of one block's round lie: found by one thread a row (two divisions' worth of arithmetic, a page, 64-bit products), read by
+// the D / 2 threads that move its pieces.  With every thread finding its own address the kernels here were bound by that: 213 instructions a warp for
+// 512 bytes, 27 us instead of XX for 65536 rows of D = 64.
+template <int ROWS>
+struct RowPlaces {
+  long long k[ROWS], v[ROWS];        // 16-byte pieces from the pools' bases; k -1: no row
+};
+template <int ROWS>
+__device__ __forceinline__ void place_row(const CacheArgs& c, RowPlaces<ROWS>& p, int row, int b, int head, int slot) {
+  const int entry = cache_page(c, slot), page = cache_page_id(c, b, entry), in_page = slot - entry * c.page_size;
+  p.k[row] = page < 0 ? -1 : page * c.k_page + head * c.k_head + in_page * c.k_slot;
+  p.v[row] = page * c.v_page + head * c.v_head + in_page * c.v_slot;
+}
+// a thread's piece of a row (of D / 2: K1, K2, V): the pool's base with the piece's offset, and which of the two places counts
+template <int D>
+struct Piece {
+  uint4* base;
+  bool is_v;
+  __device__ __forceinline__ Piece(const CacheArgs& c, int part) {
+    is_v = part >= D / 4;
+    base = is_v ? c.v + (part - D / 4) : (part < D / 8 ? c.k1 : c.k2) + (part & (D / 8 - 1));
+  }
+  template <int ROWS>
+  __device__ __forceinline__ uint4* at(const RowPlaces<ROWS>& p, int row) const {
+    return base + (is_v ? p.v[row] : p.k[row]);
+  }
+};
+
 // Stores new rows behind each sequence's last one.  Bound by HBM: 8 D bytes in and out per row.  A thread moves 16-byte pieces, neighbours
 // along a row, four rows' pieces in flight; grid (rows, b * h).
 constexpr int APPEND_THREADS = 256, APPEND_UNROLL = 4;
 
 template <int D>
 __global__ void __launch_bounds__(APPEND_THREADS) diffattn_cache_append_kernel(const CacheAppendArgs a) {
-  constexpr int PARTS = D / 2, ROWS = APPEND_THREADS / PARTS;
+  constexpr int PARTS = D / 2, ROWS = APPEND_THREADS / PARTS, BLOCK = ROWS * APPEND_UNROLL;
+  __shared__ RowPlaces<BLOCK> places;
   const CacheArgs& c = a.c;
   griddep_launch();
   const int head = blockIdx.y % c.h, b = blockIdx.y / c.h;
   const int part = threadIdx.x % PARTS;
-  const int t0 = blockIdx.x * (ROWS * APPEND_UNROLL) + threadIdx.x / PARTS;
-  const int len = cache_length(c, b), count = append_count(a, b);
+  const int first = blockIdx.x * BLOCK, row = threadIdx.x / PARTS;
+  const int count = append_count(a, b);
+  if (first >= count) return;
   const uint4* src;
   long long step;
   if (part < D / 4) {
@@ -97,27 +127,28 @@ __global__ void __launch_bounds__(APPEND_THREADS) diffattn_cache_append_kernel(c
     src = a.v + b * a.v_b + head * a.v_h + (part - D / 4);
     step = a.v_t;
   }
+  src += (first + row) * step;
   uint4 x[APPEND_UNROLL];
 #pragma unroll
   for (int i = 0; i < APPEND_UNROLL; ++i)
-    if (t0 + i * ROWS < count) x[i] = __ldg(src + (t0 + i * ROWS) * step);
-#pragma unroll
-  for (int i = 0; i < APPEND_UNROLL; ++i) {
-    const int t = t0 + i * ROWS;
-    if (t >= count) break;
-    if (t >= c.slots - len) {
-      cache_fault(kCacheFull, b, len);
-      break;
-    }
-    const int slot = len + t, p = cache_page(c, slot);
-    const int page = cache_page_id(c, b, p);
-    if (page >= 0) *cache_piece<D>(c, page, head, slot - p * c.page_size, part) = x[i];
-    if (part == 0) {
-      const long long at = (long long)blockIdx.y * c.slots + slot;
+    if (first + row + i * ROWS < count) x[i] = __ldg(src + i * ROWS * step);
+  if (threadIdx.x < BLOCK) {
+    const int t = first + threadIdx.x, len = cache_length(c, b);
+    places.k[threadIdx.x] = -1;
+    if (t < count && t < c.slots - len) {
+      place_row(c, places, threadIdx.x, b, head, len + t);
+      const long long at = (long long)blockIdx.y * c.slots + len + t;
       if (c.positions) c.positions[at] = c.next_position[b] + t;
       if (c.weights) c.weights[at] = 0.f;
+    } else if (t < count) {
+      cache_fault(kCacheFull, b, len);
     }
   }
+  __syncthreads();
+  const Piece<D> piece(c, part);
+#pragma unroll
+  for (int i = 0; i < APPEND_UNROLL; ++i)
+    if (places.k[row + i * ROWS] >= 0) *piece.at(places, row + i * ROWS) = x[i];
 }
 
 // The lengths move on once every row is stored (the kernel above reads them).

@@ -34,6 +34,7 @@ struct AttendArgs {
   int tiles_per_page;                          // 0: tiles run on over the pages; else a tile stays inside its page
   uint32_t tiles_magic;                        // ceil(2^32 / tiles_per_page), 0 for 1
   int workers;                                 // warps of the first kernel
+  int join_blocks;                             // CTAs of the second one that join
   // workspace
   int* prefix;                                 // [b + 1] tiles of the sequences before b, per head
   int* length;                                 // [b] cached tokens, before this call's
@@ -467,21 +468,14 @@ __global__ void __launch_bounds__(JT) diffattn_cache_join_kernel(const __grid_co
   constexpr int GROUPS = JT / D;               // pieces summed side by side: a thread has four of a piece's 4 D sums
   __shared__ float4 red[JT];
   __shared__ float ssq[2 * D / 32];
-  extern __shared__ int line[];                // with weights: prefix sums and lengths (a search in global memory is a chain of loads)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   griddep_wait();
   const int nb = a.c.b, heads = a.c.h;
-  if constexpr (TRACK) {
-    for (int b = threadIdx.x; b <= nb; b += JT) {
-      line[b] = a.prefix[b];
-      if (b < nb) line[nb + 1 + b] = a.length[b];
-    }
-    __syncthreads();
-  }
   const long long units = (long long)a.prefix[nb] * heads;
   const int workers = int(min((long long)a.workers, units));
   const float lam = load_lambda(a.lambda_ptr, a.lambda_dtype);
-  for (int bh = blockIdx.x; bh < nb * heads; bh += gridDim.x) {
+  // the first `a.join_blocks` CTAs join, those behind them add weights: neither chain of loads waits for the other
+  for (int bh = blockIdx.x; bh < nb * heads && blockIdx.x < a.join_blocks; bh += a.join_blocks) {
     const int b = bh / heads, head = bh - b * heads;
     const int n = a.prefix[b + 1] - a.prefix[b];
     const float gain = a.gain && threadIdx.x < 2 * D ? a.gain[threadIdx.x] : 1.f;
@@ -557,52 +551,41 @@ __global__ void __launch_bounds__(JT) diffattn_cache_join_kernel(const __grid_co
     }
   }
   if constexpr (TRACK) {
-    // the same line of tiles, cut into the warps of this grid
-    const int takers = int(min((long long)gridDim.x * (JT / 32), units));
-    const int taker = warp * int(gridDim.x) + int(blockIdx.x);
-    if (taker >= takers) return;
-    long long u = stretch_begin(units, takers, taker);
-    const long long end = stretch_begin(units, takers, taker + 1);
-    TileWalk w = walk_at(a, line, line + nb + 1, u);
-    while (u < end) {
-      const int n = int(min((long long)(w.n - w.t), end - u));      // tiles of this (sequence, head)
-      const int bh = w.b * heads + w.h;
-      int w0, w1;
-      piece_range(units, workers, u - w.t, w.n, w0, w1);
-      float* to = a.c.weights + (size_t)bh * a.c.slots;
-      constexpr int ROUND = 4;                 // tokens of a lane whose loads are under way together
-      Joined j;
-      float c1 = 0.f, c2 = 0.f;
-      for (int e0 = 0; e0 < n * T; e0 += 32 * ROUND) {      // (all lanes: they join the statistics together)
-        float s1[ROUND], s2[ROUND], old[ROUND];
-        int at[ROUND];                         // -1: no token
+    // CTA: a share of one (sequence, head)'s tokens
+    if (blockIdx.x < a.join_blocks) return;
+    const int shares = int(gridDim.x - a.join_blocks) / (nb * heads);
+    const int bh = int(blockIdx.x - a.join_blocks) % (nb * heads), share = int(blockIdx.x - a.join_blocks) / (nb * heads);
+    const int b = bh / heads, head = bh - b * heads;
+    const int p0 = a.prefix[b], n = a.prefix[b + 1] - p0, len = a.length[b];
+    if (n == 0) return;
+    const long long u = (long long)p0 * heads + (long long)head * n;
+    int w0, w1;
+    piece_range(units, workers, u, n, w0, w1);
+    const Joined j = join_stats(a.stats + bh, w0, w1, lane);
+    const float c1 = 1.f / j.l1, c2 = lam / j.l2;
+    float* to = a.c.weights + (size_t)bh * a.c.slots;
+    const float* scores = a.scores + u * 2 * T;
+    constexpr int ROUND = 4;                   // tokens of a thread whose loads are under way together
+    for (int e0 = share * JT * ROUND; e0 < n * T; e0 += shares * JT * ROUND) {
+      float s1[ROUND], s2[ROUND], old[ROUND];
+      int at[ROUND];                           // -1: no token
 #pragma unroll
-        for (int k = 0; k < ROUND; ++k) {
-          const int e = e0 + lane + 32 * k, row = e % T;
-          at[k] = -1;
-          if (e >= n * T) continue;
-          int slot, valid;
-          bool is_new;
-          attend_tile<T>(a, w.t + e / T, w.n, w.len, slot, valid, is_new);
-          if (row >= valid || slot + row >= a.c.slots) continue;
-          at[k] = slot + row;
-          const float* s = a.scores + (u + e / T) * 2 * T + row;
-          s1[k] = s[0];
-          s2[k] = s[T];
-          old[k] = is_new ? 0.f : to[at[k]];
-        }
-        if (e0 == 0) {
-          j = join_stats(a.stats + bh, w0, w1, lane);
-          c1 = 1.f / j.l1;
-          c2 = lam / j.l2;
-        }
-#pragma unroll
-        for (int k = 0; k < ROUND; ++k)
-          if (at[k] >= 0) to[at[k]] = old[k] + fabsf(ex2(s1[k] - j.m1) * c1 - ex2(s2[k] - j.m2) * c2);
+      for (int k = 0; k < ROUND; ++k) {
+        const int e = e0 + k * JT + threadIdx.x, tile = e / T, row = e % T;
+        at[k] = -1;
+        if (tile >= n) continue;
+        int slot, valid;
+        bool is_new;
+        attend_tile<T>(a, tile, n, len, slot, valid, is_new);
+        if (row >= valid || slot + row >= a.c.slots) continue;
+        at[k] = slot + row;
+        s1[k] = scores[tile * 2 * T + row];
+        s2[k] = scores[tile * 2 * T + T + row];
+        old[k] = is_new ? 0.f : to[at[k]];
       }
-      u += n;
-      w.t += n - 1;
-      if (u < end) walk_next(a, line, line + nb + 1, w);
+#pragma unroll
+      for (int k = 0; k < ROUND; ++k)
+        if (at[k] >= 0) to[at[k]] = old[k] + fabsf(ex2(s1[k] - j.m1) * c1 - ex2(s2[k] - j.m2) * c2);
     }
   }
 }

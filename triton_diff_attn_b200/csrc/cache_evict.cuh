@@ -58,37 +58,43 @@ __device__ __forceinline__ int block_before(int x, int* buf, int& total) {
   return (warp ? before : 0) + incl - x;
 }
 
-// Rows first, first + step, ... of a list of moves, UNROLL of them under way together.  Thread: one 16-byte piece of a row.
-template <int D, int THREADS, int UNROLL>
-__device__ __forceinline__ void move_rows(const EvictArgs& a, int bh, const int2* list, int count, int block, int blocks) {
-  constexpr int PARTS = D / 2, ROWS = THREADS / PARTS;
+// A list of moves, by one block of `blocks`; all its threads call it.  Thread: one 16-byte piece of a row, UNROLL rows under way together.
+constexpr int MOVE_UNROLL = 4;
+template <int D, int THREADS>
+struct MovePlaces {
+  static constexpr int PARTS = D / 2, ROWS = THREADS / PARTS, BLOCK = ROWS * MOVE_UNROLL;
+  RowPlaces<BLOCK> from, to;
+};
+template <int D, int THREADS>
+__device__ __forceinline__ void move_rows(const EvictArgs& a, MovePlaces<D, THREADS>& places, int bh, const int2* list, int count, int block, int blocks) {
+  using P = MovePlaces<D, THREADS>;
   const CacheArgs& c = a.c;
-  const int b = bh / c.h, head = bh - b * c.h, part = threadIdx.x % PARTS;
-  for (int r0 = block * (ROWS * UNROLL) + threadIdx.x / PARTS; r0 < count; r0 += blocks * (ROWS * UNROLL)) {
-    uint4 x[UNROLL];
-    uint4* to[UNROLL];
-    int2 mv[UNROLL];
-#pragma unroll
-    for (int i = 0; i < UNROLL; ++i) mv[i] = r0 + i * ROWS < count ? list[r0 + i * ROWS] : make_int2(-1, -1);
-#pragma unroll
-    for (int i = 0; i < UNROLL; ++i) {
-      to[i] = nullptr;
-      if (mv[i].x < 0) continue;
-      const int pf = cache_page(c, mv[i].x), pt = cache_page(c, mv[i].y);
-      const int from = cache_page_id(c, b, pf), dest = cache_page_id(c, b, pt);
-      if (from < 0 || dest < 0) continue;
-      x[i] = *cache_piece<D>(c, from, head, mv[i].x - pf * c.page_size, part);
-      to[i] = cache_piece<D>(c, dest, head, mv[i].y - pt * c.page_size, part);
-    }
-#pragma unroll
-    for (int i = 0; i < UNROLL; ++i) {
-      if (to[i]) *to[i] = x[i];
-      if (mv[i].x >= 0 && part == 0) {
+  const int b = bh / c.h, head = bh - b * c.h, row = threadIdx.x / P::PARTS;
+  const Piece<D> piece(c, threadIdx.x % P::PARTS);
+  for (int first = block * P::BLOCK; first < count; first += blocks * P::BLOCK) {
+    if (threadIdx.x < P::BLOCK) {
+      places.from.k[threadIdx.x] = -1;
+      if (first + threadIdx.x < count) {
+        const int2 mv = list[first + threadIdx.x];
         const long long base = (long long)bh * c.slots;
-        c.positions[base + mv[i].y] = c.positions[base + mv[i].x];
-        if (c.weights) c.weights[base + mv[i].y] = c.weights[base + mv[i].x];
+        const int pos = c.positions[base + mv.x];
+        const float w = c.weights ? c.weights[base + mv.x] : 0.f;
+        place_row(c, places.from, threadIdx.x, b, head, mv.x);
+        place_row(c, places.to, threadIdx.x, b, head, mv.y);
+        if (places.to.k[threadIdx.x] < 0) places.from.k[threadIdx.x] = -1;
+        c.positions[base + mv.y] = pos;
+        if (c.weights) c.weights[base + mv.y] = w;
       }
     }
+    __syncthreads();
+    uint4 x[MOVE_UNROLL];
+#pragma unroll
+    for (int i = 0; i < MOVE_UNROLL; ++i)
+      if (places.from.k[row + i * P::ROWS] >= 0) x[i] = *piece.at(places.from, row + i * P::ROWS);
+#pragma unroll
+    for (int i = 0; i < MOVE_UNROLL; ++i)
+      if (places.from.k[row + i * P::ROWS] >= 0) *piece.at(places.to, row + i * P::ROWS) = x[i];
+    __syncthreads();
   }
 }
 
@@ -99,6 +105,7 @@ __global__ void __launch_bounds__(SELECT_THREADS) diffattn_cache_select_kernel(c
   extern __shared__ uint32_t keys[];
   __shared__ int hist[4][256], buf[2][SELECT_WARPS];
   __shared__ int2 near_list[SELECT_LIST];
+  __shared__ MovePlaces<D, SELECT_THREADS> places;
   const CacheArgs& c = a.c;
   griddep_launch();
   const int bh = blockIdx.x, b = bh / c.h, tid = threadIdx.x, lane = tid & 31;
@@ -192,7 +199,7 @@ __global__ void __launch_bounds__(SELECT_THREADS) diffattn_cache_select_kernel(c
   }
   __syncthreads();
   if (a.moves_at_once) {
-    move_rows<D, SELECT_THREADS, 4>(a, bh, list, total, 0, 1);
+    move_rows<D, SELECT_THREADS>(a, places, bh, list, total, 0, 1);
     total = 0;
   } else if (list == near_list) {
     for (int i = tid; i < total; i += SELECT_THREADS) a.moves[(long long)bh * a.most + i] = list[i];
@@ -200,14 +207,15 @@ __global__ void __launch_bounds__(SELECT_THREADS) diffattn_cache_select_kernel(c
   if (tid == 0) a.count[bh] = total;
 }
 
-constexpr int MOVE_THREADS = 256, MOVE_UNROLL = 4;
+constexpr int MOVE_THREADS = 256;
 
 // Grid (wide, b * h): the moves that the selection wrote down.
 template <int D>
 __global__ void __launch_bounds__(MOVE_THREADS) diffattn_cache_move_kernel(const EvictArgs a) {
+  __shared__ MovePlaces<D, MOVE_THREADS> places;
   griddep_wait();
   const int bh = blockIdx.y, b = bh / a.c.h;
-  move_rows<D, MOVE_THREADS, MOVE_UNROLL>(a, bh, a.moves + (long long)bh * a.most, a.count[bh], blockIdx.x, gridDim.x);
+  move_rows<D, MOVE_THREADS>(a, places, bh, a.moves + (long long)bh * a.most, a.count[bh], blockIdx.x, gridDim.x);
   if (blockIdx.x == 0 && bh == b * a.c.h && threadIdx.x == 0 && a.c.lengths[b] > a.keep) a.c.lengths[b] = a.keep;
 }
 

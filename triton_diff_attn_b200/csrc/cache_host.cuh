@@ -153,13 +153,13 @@ int attend_launch(const DiffAttnCacheParams* p, da::AttendArgs& a) {
   const int sms = sm_count(p->device);
   if ((rc = launch(kernel, dim3(sms), da::attend::Geo<D>::THREADS, smem, stream, false, k1, k2, v, a))) return rc;
   // 1024 threads for more than a dozen pieces a (sequence, head): B1 H16 N16384 D64 (74 pieces) XX us instead of XX
-  const int bh = p->B * p->H, line = TRACK ? 4 * (2 * p->B + 1) : 0;
+  const int bh = p->B * p->H;
   if (a.workers > 12 * bh) {
-    const int grid = TRACK ? sms * 2 : std::min(bh, sms * 2);
-    return launch(da::diffattn_cache_join_kernel<D, 1024, BF, TRACK>, dim3(grid), 1024, line, stream, true, a);
+    a.join_blocks = std::min(bh, sms * 2);
+    return launch(da::diffattn_cache_join_kernel<D, 1024, BF, TRACK>, dim3(a.join_blocks + (TRACK ? bh * ((sms + bh - 1) / bh) : 0)), 1024, 0, stream, true, a);
   }
-  const int grid = TRACK ? sms * 4 : std::min(bh, sms * 8);
-  return launch(da::diffattn_cache_join_kernel<D, 256, BF, TRACK>, dim3(grid), 256, line, stream, true, a);
+  a.join_blocks = std::min(bh, sms * 8);
+  return launch(da::diffattn_cache_join_kernel<D, 256, BF, TRACK>, dim3(a.join_blocks + (TRACK ? bh * ((4 * sms + bh - 1) / bh) : 0)), 256, 0, stream, true, a);
 }
 template <int D>
 int attend_launch(const DiffAttnCacheParams* p, da::AttendArgs& a) {
@@ -178,7 +178,7 @@ int evict_launch(const DiffAttnCacheParams* p, const da::EvictArgs& a) {
   if (a.moves_at_once)
     return launch(da::diffattn_cache_shorten_kernel, dim3((p->B + da::MOVE_THREADS - 1) / da::MOVE_THREADS), da::MOVE_THREADS, 0, stream, true, a);
   // as many CTAs as the SMs hold, spread over the (sequence, head)s, but no more than there can be moves for
-  const int rows = da::MOVE_THREADS / (D / 2) * da::MOVE_UNROLL;
+  const int rows = da::MovePlaces<D, da::MOVE_THREADS>::BLOCK;
   const int wide = std::max(1, std::min((a.most + rows - 1) / rows, (sm_count(p->device) * 8 + bh - 1) / bh));
   return launch(da::diffattn_cache_move_kernel<D>, dim3(wide, bh), da::MOVE_THREADS, 0, stream, true, a);
 }
