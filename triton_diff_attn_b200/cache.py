@@ -19,15 +19,28 @@ from .layers import _IO_DTYPES, _LAMBDA_DTYPES, EPS
 def _addressable(t) -> bool:
     """Rows the kernels can read as they lie: unit stride in the last dimension, the other strides positive multiples of 8 elements
     (a dimension of one element has none), base pointer 16-byte aligned."""
-    return (t.data_ptr() % 16 == 0 and (t.stride(-1) == 1 or t.shape[-1] == 1)
+    return (t.data_ptr() % 16 == 0 and t.stride(-1) == 1
             and all(n <= 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:-1], t.stride()[:-1])))
 
 
+def _rows(t):
+    """`t` and its strides where its rows can be read as they lie, else a copy."""
+    sb, sh, st, sd = strides = t.stride()
+    if sd == 1 and sb > 0 and sh > 0 and st > 0 and not (sb | sh | st) % 8 and not t.data_ptr() % 16:
+        return t, strides          # (the common case: what the general rule would say)
+    if not _addressable(t):
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.stride()
+
+
 def _pair(a, b):
-    """Two tensors of one shape with the same strides; copied where they differ or cannot be addressed."""
-    if a.stride() == b.stride() and _addressable(a) and _addressable(b):
-        return a, b
-    return a.clone(memory_format=torch.contiguous_format), b.clone(memory_format=torch.contiguous_format)
+    """Two tensors of one shape with the same strides, and these; copied where they differ or cannot be addressed."""
+    a, sa = _rows(a)
+    b, sb = _rows(b)
+    if sa != sb:
+        a, b = a.clone(memory_format=torch.contiguous_format), b.clone(memory_format=torch.contiguous_format)
+        sa = a.stride()
+    return a, b, sa
 
 
 class DiffAttnCache:
@@ -124,6 +137,7 @@ class DiffAttnCache:
         self._k1_pages, self._k2_pages, self._v_pages, self._page_table = k1_pages, k2_pages, v_pages, page_table
         self._lengths, self._positions, self._next_position, self._weights = lengths, positions, next_position, weights
         self._shape = (batch, heads, d)
+        self._device, self._index, self._dtype = device, k1_pages.get_device(), k1_pages.dtype
         p = _lib.DiffAttnCacheParams()
         p.struct_size = C.sizeof(p)
         p.device = k1_pages.get_device()
@@ -135,6 +149,7 @@ class DiffAttnCache:
         p.table_stride = page_table.stride(0)
         p.sm_scale, p.eps = 1.0 / math.sqrt(d), EPS
         self._sizes = p
+        self._attend_bytes = int(_lib.lib.diffattn_cache_workspace_bytes(self._params(), _lib.CACHE_ATTEND))
 
     k1_pages = property(lambda self: self._k1_pages)
     k2_pages = property(lambda self: self._k2_pages)
@@ -159,12 +174,15 @@ class DiffAttnCache:
 
     def _check(self, name, t, rows, width):
         batch, heads, _ = self._shape
+        if (isinstance(t, torch.Tensor) and t.dtype is self._dtype and t.get_device() == self._index and t.shape == (batch, heads, rows, width)
+                and not t.requires_grad):
+            return
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} must be a tensor")
-        if t.device != self._k1_pages.device:
-            raise RuntimeError(f"{name} is on {t.device}, the cache on {self._k1_pages.device}")
-        if t.dtype != self._k1_pages.dtype:
-            raise ValueError(f"{name} is {t.dtype}, the cache {self._k1_pages.dtype}")
+        if t.device != self._device:
+            raise RuntimeError(f"{name} is on {t.device}, the cache on {self._device}")
+        if t.dtype != self._dtype:
+            raise ValueError(f"{name} is {t.dtype}, the cache {self._dtype}")
         if tuple(t.shape) != (batch, heads, rows, width):
             raise ValueError(f"{name} shape {tuple(t.shape)} != {(batch, heads, rows, width)}")
         if t.requires_grad and torch.is_grad_enabled():
@@ -172,19 +190,18 @@ class DiffAttnCache:
 
     def _tokens(self, p, k1, k2, v, rows):
         d = self._shape[2]
-        for name, t, width in (("k1", k1, d), ("k2", k2, d), ("v", v, 2 * d)):
-            self._check(name, t, rows, width)
-        k1, k2 = _pair(k1, k2)
-        if not _addressable(v):
-            v = v.clone(memory_format=torch.contiguous_format)
+        self._check("k1", k1, rows, d)
+        self._check("k2", k2, rows, d)
+        self._check("v", v, rows, 2 * d)
+        k1, k2, sk = _pair(k1, k2)
+        v, sv = _rows(v)
         p.k1, p.k2, p.v = k1.data_ptr(), k2.data_ptr(), v.data_ptr()
-        p.k_stride_b, p.k_stride_h, p.k_stride_t, _ = k1.stride()
-        p.v_stride_b, p.v_stride_h, p.v_stride_t, _ = v.stride()
+        p.k_stride_b, p.k_stride_h, p.k_stride_t, _ = sk
+        p.v_stride_b, p.v_stride_h, p.v_stride_t, _ = sv
         return k1, k2, v
 
-    def _workspace(self, p, operation):
-        nbytes = int(_lib.lib.diffattn_cache_workspace_bytes(p, operation))
-        ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=self._k1_pages.device)
+    def _workspace(self, p, nbytes):
+        ws = self._lengths.new_empty(max(nbytes, 256) // 4)
         p.workspace, p.workspace_bytes = ws.data_ptr(), nbytes
         return ws
 
@@ -203,11 +220,12 @@ class DiffAttnCache:
         if counts is not None:
             if not isinstance(counts, torch.Tensor):
                 raise TypeError("counts must be a tensor")
-            if counts.device != self._k1_pages.device:
-                raise RuntimeError(f"counts is on {counts.device}, the cache on {self._k1_pages.device}")
+            if counts.get_device() != self._index:
+                raise RuntimeError(f"counts is on {counts.device}, the cache on {self._device}")
             if counts.dtype not in (torch.int32, torch.int64) or tuple(counts.shape) != (self._shape[0],):
                 raise ValueError(f"counts must be int32 or int64 of shape {(self._shape[0],)}")
-            counts = counts.to(torch.int32).contiguous()
+            if counts.dtype is not torch.int32 or not counts.is_contiguous():
+                counts = counts.to(torch.int32).contiguous()
             p.counts = counts.data_ptr()
         _lib.check(_lib.lib.diffattn_cache_append(p), "diffattn_cache_append")
 
@@ -220,37 +238,40 @@ class DiffAttnCache:
         A cache with `weights` adds |P1 - lambda P2| to each token's.
 
         A sequence that is not in use has length 0; a step stores a token there like everywhere (set its length back to 0 if that matters)."""
-        d = self._shape[2]
+        batch, heads, d = self._shape
         self._check("q1", q1, 1, d)
         self._check("q2", q2, 1, d)
-        if not isinstance(lambda_scale, torch.Tensor):
-            raise TypeError("lambda_scale must be a 1-element CUDA tensor")
-        if lambda_scale.numel() != 1 or lambda_scale.dtype not in _LAMBDA_DTYPES:
-            raise ValueError("lambda_scale must hold one float16, bfloat16 or float32 element")
-        dev = self._k1_pages.device
-        if lambda_scale.device != dev:
-            raise RuntimeError(f"lambda_scale is on {lambda_scale.device}, the cache on {dev}")
-        if torch.is_grad_enabled() and (lambda_scale.requires_grad or (isinstance(gain, torch.Tensor) and gain.requires_grad)):
-            raise RuntimeError("lambda_scale or gain requires a gradient, and the cache has no backward pass: call it under torch.no_grad()")
+        lam = lambda_scale
+        if not (isinstance(lam, torch.Tensor) and lam.get_device() == self._index and lam.numel() == 1 and lam.dtype in _LAMBDA_DTYPES):
+            self._refuse_lambda(lam)
         if gain is not None:
-            if not isinstance(gain, torch.Tensor) or gain.device != dev or tuple(gain.shape) != (2 * d,) or not gain.is_floating_point():
+            if not isinstance(gain, torch.Tensor) or gain.get_device() != self._index or gain.shape != (2 * d,) or not gain.is_floating_point():
                 raise ValueError("gain must be a floating-point tensor of shape [2*D] on the cache's device")
-            gain = gain.detach().to(torch.float32).contiguous()
+        if (lam.requires_grad or (gain is not None and gain.requires_grad)) and torch.is_grad_enabled():
+            raise RuntimeError("lambda_scale or gain requires a gradient, and the cache has no backward pass: call it under torch.no_grad()")
         p = self._params()
         if k1 is not None or k2 is not None or v is not None:
-            keep = self._tokens(p, k1, k2, v, 1)  # noqa: F841
-        q1, q2 = _pair(q1, q2)
-        p.q1, p.q2 = q1.data_ptr(), q2.data_ptr()
-        p.q_stride_b, p.q_stride_h, _, _ = q1.stride()
-        p.lambda_scale, p.lambda_dtype = lambda_scale.data_ptr(), _LAMBDA_DTYPES[lambda_scale.dtype]
+            keep = self._tokens(p, k1, k2, v, 1)  # noqa: F841  (copies stay until the call is enqueued)
+        q1, q2, sq = _pair(q1, q2)
+        p.q1, p.q2, p.q_stride_b, p.q_stride_h = q1.data_ptr(), q2.data_ptr(), sq[0], sq[1]
+        p.lambda_scale, p.lambda_dtype = lam.data_ptr(), _LAMBDA_DTYPES[lam.dtype]
         p.rms_norm, p.lambda_init = 1 if rms_norm else 0, float(lambda_init)
         if gain is not None:
+            if gain.dtype is not torch.float32 or gain.stride(0) != 1:
+                gain = gain.detach().to(torch.float32).contiguous()
             p.gain = gain.data_ptr()
-        y = torch.empty((*self._shape[:2], 1, 2 * d), dtype=q1.dtype, device=dev)
+        y = self._k1_pages.new_empty((batch, heads, 1, 2 * d))
         p.y = y.data_ptr()
-        ws = self._workspace(p, _lib.CACHE_ATTEND)  # noqa: F841
+        ws = self._workspace(p, self._attend_bytes)  # noqa: F841
         _lib.check(_lib.lib.diffattn_cache_attend(p), "diffattn_cache_attend")
         return y
+
+    def _refuse_lambda(self, lam):
+        if not isinstance(lam, torch.Tensor):
+            raise TypeError("lambda_scale must be a 1-element CUDA tensor")
+        if lam.numel() != 1 or lam.dtype not in _LAMBDA_DTYPES:
+            raise ValueError("lambda_scale must hold one float16, bfloat16 or float32 element")
+        raise RuntimeError(f"lambda_scale is on {lam.device}, the cache on {self._device}")
 
     def evict(self, keep: int, recent: int = 0) -> None:
         """Cuts every sequence longer than `keep` back to `keep` tokens, per head: the tokens of its last `recent` positions stay, then those with
@@ -259,5 +280,5 @@ class DiffAttnCache:
         Pages behind the new lengths are free again."""
         p = self._params()
         p.keep, p.recent = int(keep), int(recent)
-        ws = self._workspace(p, _lib.CACHE_EVICT)  # noqa: F841
+        ws = self._workspace(p, int(_lib.lib.diffattn_cache_workspace_bytes(p, _lib.CACHE_EVICT)))  # noqa: F841
         _lib.check(_lib.lib.diffattn_cache_evict(p), "diffattn_cache_evict")

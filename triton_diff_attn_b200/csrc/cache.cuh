@@ -50,12 +50,13 @@ __device__ __forceinline__ int cache_page(const CacheArgs& c, int slot) {
   return p;
 }
 // the page behind entry `i` of sequence b's table, or -1
-__device__ __forceinline__ int cache_page_id(const CacheArgs& c, int b, int i) {
-  const int id = __ldg(c.page_table + b * c.table_stride + i);
+__device__ __forceinline__ int cache_page_load(const CacheArgs& c, int b, int i) { return __ldg(c.page_table + b * c.table_stride + i); }
+__device__ __forceinline__ int cache_page_check(const CacheArgs& c, int b, int i, int id) {
   if (uint32_t(id) < uint32_t(c.num_pages)) return id;
   cache_fault(kCacheBadPage, b, i);
   return -1;
 }
+__device__ __forceinline__ int cache_page_id(const CacheArgs& c, int b, int i) { return cache_page_check(c, b, i, cache_page_load(c, b, i)); }
 
 // The 16-byte piece `part` (of D / 2: K1, then K2, then V) of a cached row.
 template <int D>
@@ -82,9 +83,10 @@ template <int ROWS>
 struct RowPlaces {
   long long k[ROWS], v[ROWS];        // 16-byte pieces from the pools' bases; k -1: no row
 };
+// (`id`: what the page table holds for the slot; the caller has loaded it, so that two of them are under way together)
 template <int ROWS>
-__device__ __forceinline__ void place_row(const CacheArgs& c, RowPlaces<ROWS>& p, int row, int b, int head, int slot) {
-  const int entry = cache_page(c, slot), page = cache_page_id(c, b, entry), in_page = slot - entry * c.page_size;
+__device__ __forceinline__ void place_row(const CacheArgs& c, RowPlaces<ROWS>& p, int row, int b, int head, int slot, int entry, int id) {
+  const int page = cache_page_check(c, b, entry, id), in_page = slot - entry * c.page_size;
   p.k[row] = page < 0 ? -1 : page * c.k_page + head * c.k_head + in_page * c.k_slot;
   p.v[row] = page * c.v_page + head * c.v_head + in_page * c.v_slot;
 }
@@ -136,7 +138,8 @@ __global__ void __launch_bounds__(APPEND_THREADS) diffattn_cache_append_kernel(c
     const int t = first + threadIdx.x, len = cache_length(c, b);
     places.k[threadIdx.x] = -1;
     if (t < count && t < c.slots - len) {
-      place_row(c, places, threadIdx.x, b, head, len + t);
+      const int entry = cache_page(c, len + t);
+      place_row(c, places, threadIdx.x, b, head, len + t, entry, cache_page_load(c, b, entry));
       const long long at = (long long)blockIdx.y * c.slots + len + t;
       if (c.positions) c.positions[at] = c.next_position[b] + t;
       if (c.weights) c.weights[at] = 0.f;

@@ -36,7 +36,7 @@ struct AttendArgs {
   int workers;                                 // warps of the first kernel
   int join_blocks;                             // CTAs of the second one that join
   // workspace
-  int* prefix;                                 // [b + 1] tiles of the sequences before b, per head
+  int* prefix;                                 // [b + 2] tiles of the sequences before b, per head; at the end the workers that have any
   int* length;                                 // [b] cached tokens, before this call's
   int* position;                               // [b] the new token's position
   float4* stats;                               // [workers + b * h] {m1, l1, m2, l2} of a piece
@@ -208,11 +208,16 @@ diffattn_cache_attend_kernel(const __grid_constant__ CUtensorMap tm_k1, const __
   for (int b = b0; b < b1; ++b) prefix[b + 1] += before;
   if (threadIdx.x == 0) prefix[0] = 0;
   __syncthreads();
-  if (blockIdx.x == 0)
-    for (int b = threadIdx.x; b <= nb; b += THREADS) a.prefix[b] = prefix[b];
-
+  // Each worker's piece costs the joining kernel about 1 / 80 of what a tile costs here (a CTA joins them, four rounds of loads for 64), so with
+  // very few heads more than sqrt(80 tiles heads) workers lose more there than they gain: B1 H1 N16384 D64 XX -> XX us
   const long long units = (long long)prefix[nb] * a.c.h;
-  const int workers = int(min((long long)a.workers, units));
+  const int most = int(min((long long)a.workers, units)), best = int(sqrtf(80.f * float(units) * float(nb * a.c.h)));
+  const int workers = units > 0 ? max(min(most, best), 1) : 0;
+  if (blockIdx.x == 0) {
+    for (int b = threadIdx.x; b <= nb; b += THREADS) a.prefix[b] = prefix[b];
+    if (threadIdx.x == 0) a.prefix[nb + 1] = workers;
+  }
+
   const int worker = warp * int(gridDim.x) + int(blockIdx.x);      // few tiles: one to a CTA before any CTA has two
   if (worker >= workers) return;
   const long long first = stretch_begin(units, workers, worker);
@@ -443,151 +448,235 @@ __device__ __forceinline__ void join(float& m, float& l, float m2, float l2) {
   l = l * ex2(m - top) + l2 * ex2(m2 - top);
   m = top;
 }
-__device__ __forceinline__ Joined join_stats(const float4* stats, int w0, int w1, int lane) {      // a whole warp
-  Joined j{-3e38f, 0.f, -3e38f, 0.f};
-  for (int w = w0 + lane; w <= w1; w += 32) {
-    const float4 x = stats[w];
-    join(j.m1, j.l1, x.x, x.y);
-    join(j.m2, j.l2, x.z, x.w);
-  }
+__device__ __forceinline__ void join_lanes(Joined& j) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     join(j.m1, j.l1, __shfl_xor_sync(0xffffffffu, j.m1, o), __shfl_xor_sync(0xffffffffu, j.l1, o));
     join(j.m2, j.l2, __shfl_xor_sync(0xffffffffu, j.m2, o), __shfl_xor_sync(0xffffffffu, j.l2, o));
   }
+}
+__device__ __forceinline__ Joined join_stats(const float4* stats, int first, int last, int step, int lane) {      // a whole warp: pieces first + lane, ...
+  Joined j{-3e38f, 0.f, -3e38f, 0.f};
+#pragma unroll 2
+  for (int w = first + lane; w <= last; w += step) {
+    const float4 x = stats[w];
+    join(j.m1, j.l1, x.x, x.y);
+    join(j.m2, j.l2, x.z, x.w);
+  }
+  join_lanes(j);
   return j;
 }
 
-// Many threads where a (sequence, head) has many pieces (few of them share the workers): what counts is the chain of loads, prefix, statistics,
-// sums, each about 0.7 us away in L2, so all of a thread's loads go out together and there are enough threads to need one round of them.
-constexpr int JOIN_AHEAD = 4;                  // pieces whose sums a thread requests before it knows their weights
+// What a call leaves behind besides y, for (sequence, head) bh; one thread.
+__device__ __forceinline__ void join_finish(const AttendArgs& a, int bh, int b, int head) {
+  if (a.nk1 == nullptr) return;
+  const int len = a.length[b];
+  if (len < a.c.slots) {
+    if (a.c.positions) a.c.positions[(size_t)bh * a.c.slots + len] = a.position[b];
+    if (head == 0) {
+      a.c.lengths[b] = len + 1;
+      if (a.c.next_position) a.c.next_position[b] = a.position[b] + 1;
+    }
+  } else {
+    if (head == 0) a.c.lengths[b] = len;
+    cache_fault(kCacheFull, b, len);
+  }
+}
+
+// The weights of a share of one (sequence, head)'s tokens; a CTA of JT threads.
+template <int T, int JT>
+__device__ __forceinline__ void join_weights(const AttendArgs& a, int bh, int share, int shares) {
+  const int heads = a.c.h, b = bh / heads, head = bh - b * heads, lane = threadIdx.x & 31;
+  const int p0 = a.prefix[b], n = a.prefix[b + 1] - p0, len = a.length[b];
+  const long long units = (long long)a.prefix[a.c.b] * heads;
+  if (n == 0) return;
+  const int workers = a.prefix[a.c.b + 1];
+  const float lam = load_lambda(a.lambda_ptr, a.lambda_dtype);
+  const long long u = (long long)p0 * heads + (long long)head * n;
+  int w0, w1;
+  piece_range(units, workers, u, n, w0, w1);
+  const Joined j = join_stats(a.stats + bh, w0, w1, 32, lane);
+  const float c1 = 1.f / j.l1, c2 = lam / j.l2;
+  float* to = a.c.weights + (size_t)bh * a.c.slots;
+  const float* scores = a.scores + u * 2 * T;
+  constexpr int ROUND = 4;                     // tokens of a thread whose loads are under way together
+  for (int t0 = share * (JT / T) * ROUND; t0 < n; t0 += shares * (JT / T) * ROUND) {
+    float s1[ROUND], s2[ROUND], old[ROUND];
+    int at[ROUND];                             // -1: no token
+#pragma unroll
+    for (int k = 0; k < ROUND; ++k) {
+      const int tile = t0 + (k * JT + int(threadIdx.x)) / T, row = threadIdx.x % T;
+      at[k] = -1;
+      if (tile >= n) continue;
+      int slot, valid;
+      bool is_new;
+      attend_tile<T>(a, tile, n, len, slot, valid, is_new);
+      if (row >= valid || slot + row >= a.c.slots) continue;
+      at[k] = slot + row;
+      s1[k] = scores[(long long)tile * 2 * T + row];
+      s2[k] = scores[(long long)tile * 2 * T + T + row];
+      old[k] = is_new ? 0.f : to[at[k]];
+    }
+#pragma unroll
+    for (int k = 0; k < ROUND; ++k)
+      if (at[k] >= 0) to[at[k]] = old[k] + fabsf(ex2(s1[k] - j.m1) * c1 - ex2(s2[k] - j.m2) * c2);
+  }
+}
+
+// Two forms.  What counts is the chain of loads, prefix sums, statistics, sums, each about 0.7 us away in L2.  Several pieces a (sequence, head):
+// JT threads join them, so that all loads of a round go out together.  Few: a warp does, without a barrier, and a CTA holds eight.
+// In both the first `a.join_blocks` CTAs join and those behind them add weights: neither chain waits for the other.
+constexpr int JOIN_FEW = 256;
 
 template <int D, int JT, bool BF, bool TRACK>
 __global__ void __launch_bounds__(JT) diffattn_cache_join_kernel(const __grid_constant__ AttendArgs a) {
   constexpr int T = attend::Geo<D>::T;
-  constexpr int GROUPS = JT / D;               // pieces summed side by side: a thread has four of a piece's 4 D sums
+  constexpr int GROUPS = JT / D;        // pieces summed side by side: a thread has four of a piece's 4 D sums
+  constexpr int AHEAD = 4;                     // pieces whose sums a thread requests before it knows their weights
   __shared__ float4 red[JT];
+  __shared__ Joined part[JT / 32];
   __shared__ float ssq[2 * D / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   griddep_wait();
   const int nb = a.c.b, heads = a.c.h;
+  if (int(blockIdx.x) >= a.join_blocks) {
+    if constexpr (TRACK) {
+      const int at = int(blockIdx.x) - a.join_blocks;
+      join_weights<T, JT>(a, at % (nb * heads), at / (nb * heads), int(gridDim.x - a.join_blocks) / (nb * heads));
+    }
+    return;
+  }
   const long long units = (long long)a.prefix[nb] * heads;
-  const int workers = int(min((long long)a.workers, units));
+  const int workers = a.prefix[nb + 1];
   const float lam = load_lambda(a.lambda_ptr, a.lambda_dtype);
-  // the first `a.join_blocks` CTAs join, those behind them add weights: neither chain of loads waits for the other
-  for (int bh = blockIdx.x; bh < nb * heads && blockIdx.x < a.join_blocks; bh += a.join_blocks) {
-    const int b = bh / heads, head = bh - b * heads;
-    const int n = a.prefix[b + 1] - a.prefix[b];
-    const float gain = a.gain && threadIdx.x < 2 * D ? a.gain[threadIdx.x] : 1.f;
-    float out = 0.f;
-    if (n > 0) {
-      int w0, w1;
-      piece_range(units, workers, (long long)a.prefix[b] * heads + (long long)head * n, n, w0, w1);
-      const float4* stats = a.stats + bh;
-      const int col = threadIdx.x % D, group = threadIdx.x / D;
-      const bool second = col >= D / 2;
-      const float4* acc = a.acc + (size_t)bh * D + col;
-      float4 x[JOIN_AHEAD];
-      float mx[JOIN_AHEAD];
-#pragma unroll
-      for (int k = 0; k < JOIN_AHEAD; ++k) {
-        const int w = w0 + group + k * GROUPS;
-        mx[k] = -INFINITY;
-        x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (w <= w1) {
-          x[k] = acc[(size_t)w * D];
-          mx[k] = second ? stats[w].z : stats[w].x;
-        }
-      }
-      const Joined j = join_stats(stats, w0, w1, lane);
-      const float top = second ? j.m2 : j.m1;
-      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-      auto add = [&](const float4& v, float m) {
-        const float c = ex2(m - top);
-        sum.x += c * v.x; sum.y += c * v.y; sum.z += c * v.z; sum.w += c * v.w;
-      };
-#pragma unroll
-      for (int k = 0; k < JOIN_AHEAD; ++k)
-        if (w0 + group + k * GROUPS <= w1) add(x[k], mx[k]);
-#pragma unroll 4
-      for (int w = w0 + group + JOIN_AHEAD * GROUPS; w <= w1; w += GROUPS) add(acc[(size_t)w * D], second ? stats[w].z : stats[w].x);
-      red[threadIdx.x] = sum;
-      __syncthreads();
-      if (threadIdx.x < 2 * D) {
-        const float* r = reinterpret_cast<const float*>(red);
-        float o1 = 0.f, o2 = 0.f;
-#pragma unroll
-        for (int g = 0; g < GROUPS; ++g) {
-          o1 += r[g * 4 * D + threadIdx.x];
-          o2 += r[g * 4 * D + 2 * D + threadIdx.x];
-        }
-        out = o1 / j.l1 - lam * (o2 / j.l2);
-        float sq = out * out;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
-        if (lane == 0) ssq[warp] = sq;
-      }
-      __syncthreads();
-      if (a.rms_norm) {
-        float sq = 0.f;
-#pragma unroll
-        for (int k = 0; k < 2 * D / 32; ++k) sq += ssq[k];
-        out *= rsqrtf(sq / float(2 * D) + a.eps) * a.out_scale;
-      }
-    }
-    if (threadIdx.x < 2 * D) a.y[size_t(bh) * 2 * D + threadIdx.x] = from_float16b<BF>(out * gain);
-    if (a.nk1 && threadIdx.x == 0) {
-      const int len = a.length[b];
-      if (len < a.c.slots) {
-        if (a.c.positions) a.c.positions[(size_t)bh * a.c.slots + len] = a.position[b];
-        if (head == 0) {
-          a.c.lengths[b] = len + 1;
-          if (a.c.next_position) a.c.next_position[b] = a.position[b] + 1;
-        }
-      } else {
-        if (head == 0) a.c.lengths[b] = len;
-        cache_fault(kCacheFull, b, len);
-      }
-    }
-  }
-  if constexpr (TRACK) {
-    // CTA: a share of one (sequence, head)'s tokens
-    if (blockIdx.x < a.join_blocks) return;
-    const int shares = int(gridDim.x - a.join_blocks) / (nb * heads);
-    const int bh = int(blockIdx.x - a.join_blocks) % (nb * heads), share = int(blockIdx.x - a.join_blocks) / (nb * heads);
-    const int b = bh / heads, head = bh - b * heads;
-    const int p0 = a.prefix[b], n = a.prefix[b + 1] - p0, len = a.length[b];
-    if (n == 0) return;
-    const long long u = (long long)p0 * heads + (long long)head * n;
+  const int bh = blockIdx.x, b = bh / heads, head = bh - b * heads;
+  const int n = a.prefix[b + 1] - a.prefix[b];
+  const float gain = a.gain && threadIdx.x < 2 * D ? a.gain[threadIdx.x] : 1.f;
+  float out = 0.f;
+  if (n > 0) {
     int w0, w1;
-    piece_range(units, workers, u, n, w0, w1);
-    const Joined j = join_stats(a.stats + bh, w0, w1, lane);
-    const float c1 = 1.f / j.l1, c2 = lam / j.l2;
-    float* to = a.c.weights + (size_t)bh * a.c.slots;
-    const float* scores = a.scores + u * 2 * T;
-    constexpr int ROUND = 4;                   // tokens of a thread whose loads are under way together
-    for (int e0 = share * JT * ROUND; e0 < n * T; e0 += shares * JT * ROUND) {
-      float s1[ROUND], s2[ROUND], old[ROUND];
-      int at[ROUND];                           // -1: no token
+    piece_range(units, workers, (long long)a.prefix[b] * heads + (long long)head * n, n, w0, w1);
+    const float4* stats = a.stats + bh;
+    const int col = threadIdx.x % D, group = threadIdx.x / D;
+    const bool second = col >= D / 2;
+    const float4* acc = a.acc + (size_t)bh * D + col;
+    float4 x[AHEAD];
+    float mx[AHEAD];
 #pragma unroll
-      for (int k = 0; k < ROUND; ++k) {
-        const int e = e0 + k * JT + threadIdx.x, tile = e / T, row = e % T;
-        at[k] = -1;
-        if (tile >= n) continue;
-        int slot, valid;
-        bool is_new;
-        attend_tile<T>(a, tile, n, len, slot, valid, is_new);
-        if (row >= valid || slot + row >= a.c.slots) continue;
-        at[k] = slot + row;
-        s1[k] = scores[tile * 2 * T + row];
-        s2[k] = scores[tile * 2 * T + T + row];
-        old[k] = is_new ? 0.f : to[at[k]];
+    for (int k = 0; k < AHEAD; ++k) {
+      const int w = w0 + group + k * GROUPS;
+      if (w <= w1) {
+        x[k] = acc[(size_t)w * D];
+        mx[k] = second ? stats[w].z : stats[w].x;
       }
+    }
+    Joined j = join_stats(stats, w0 + warp * 32, w1, JT, lane);
+    if (lane == 0) part[warp] = j;
+    __syncthreads();
+    j = lane < JT / 32 ? part[lane] : Joined{-3e38f, 0.f, -3e38f, 0.f};
+    join_lanes(j);
+    const float top = second ? j.m2 : j.m1;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](const float4& v, float m) {
+      const float c = ex2(m - top);
+      sum.x += c * v.x; sum.y += c * v.y; sum.z += c * v.z; sum.w += c * v.w;
+    };
 #pragma unroll
-      for (int k = 0; k < ROUND; ++k)
-        if (at[k] >= 0) to[at[k]] = old[k] + fabsf(ex2(s1[k] - j.m1) * c1 - ex2(s2[k] - j.m2) * c2);
+    for (int k = 0; k < AHEAD; ++k)
+      if (w0 + group + k * GROUPS <= w1) add(x[k], mx[k]);
+#pragma unroll 4
+    for (int w = w0 + group + AHEAD * GROUPS; w <= w1; w += GROUPS) add(acc[(size_t)w * D], second ? stats[w].z : stats[w].x);
+    red[threadIdx.x] = sum;
+    __syncthreads();
+    if (threadIdx.x < 2 * D) {
+      const float* r = reinterpret_cast<const float*>(red);
+      float o1 = 0.f, o2 = 0.f;
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) {
+        o1 += r[g * 4 * D + threadIdx.x];
+        o2 += r[g * 4 * D + 2 * D + threadIdx.x];
+      }
+      out = o1 / j.l1 - lam * (o2 / j.l2);
+      float sq = out * out;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+      if (lane == 0) ssq[warp] = sq;
+    }
+    __syncthreads();
+    if (a.rms_norm) {
+      float sq = 0.f;
+#pragma unroll
+      for (int k = 0; k < 2 * D / 32; ++k) sq += ssq[k];
+      out *= rsqrtf(sq / float(2 * D) + a.eps) * a.out_scale;
     }
   }
+  if (threadIdx.x < 2 * D) a.y[size_t(bh) * 2 * D + threadIdx.x] = from_float16b<BF>(out * gain);
+  if (threadIdx.x == 0) join_finish(a, bh, b, head);
+}
+
+template <int D, bool BF, bool TRACK>
+__global__ void __launch_bounds__(JOIN_FEW) diffattn_cache_join_few_kernel(const __grid_constant__ AttendArgs a) {
+  constexpr int T = attend::Geo<D>::T;
+  constexpr int C = 2 * D / 32;                // value columns of a lane, neighbours: 2, 4 or 8
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  griddep_wait();
+  const int nb = a.c.b, heads = a.c.h;
+  if (int(blockIdx.x) >= a.join_blocks) {
+    if constexpr (TRACK) {
+      const int at = int(blockIdx.x) - a.join_blocks;
+      join_weights<T, JOIN_FEW>(a, at % (nb * heads), at / (nb * heads), int(gridDim.x - a.join_blocks) / (nb * heads));
+    }
+    return;
+  }
+  const int bh = blockIdx.x * (JOIN_FEW / 32) + warp;
+  if (bh >= nb * heads) return;
+  const long long units = (long long)a.prefix[nb] * heads;
+  const int workers = a.prefix[nb + 1];
+  const float lam = load_lambda(a.lambda_ptr, a.lambda_dtype);
+  const int b = bh / heads, head = bh - b * heads;
+  const int n = a.prefix[b + 1] - a.prefix[b];
+  float out[C];
+#pragma unroll
+  for (int k = 0; k < C; ++k) out[k] = 0.f;
+  if (n > 0) {
+    int w0, w1;
+    piece_range(units, workers, (long long)a.prefix[b] * heads + (long long)head * n, n, w0, w1);
+    const float4* stats = a.stats + bh;
+    const float* acc = reinterpret_cast<const float*>(a.acc + (size_t)bh * D) + lane * C;
+    const Joined j = join_stats(stats, w0, w1, 32, lane);
+    float o1[C], o2[C];
+#pragma unroll
+    for (int k = 0; k < C; ++k) o1[k] = o2[k] = 0.f;
+#pragma unroll 4
+    for (int w = w0; w <= w1; ++w) {
+      const float c1 = ex2(stats[w].x - j.m1), c2 = ex2(stats[w].z - j.m2);
+      const float* x = acc + (size_t)w * 4 * D;
+#pragma unroll
+      for (int k = 0; k < C; k += 2) {
+        const float2 p = *reinterpret_cast<const float2*>(x + k), q = *reinterpret_cast<const float2*>(x + 2 * D + k);
+        o1[k] += c1 * p.x; o1[k + 1] += c1 * p.y;
+        o2[k] += c2 * q.x; o2[k + 1] += c2 * q.y;
+      }
+    }
+    float sq = 0.f;
+#pragma unroll
+    for (int k = 0; k < C; ++k) {
+      out[k] = o1[k] / j.l1 - lam * (o2[k] / j.l2);
+      sq += out[k] * out[k];
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+    const float scale = a.rms_norm ? rsqrtf(sq / float(2 * D) + a.eps) * a.out_scale : 1.f;
+#pragma unroll
+    for (int k = 0; k < C; ++k) out[k] *= scale;
+  }
+  uint32_t* y = reinterpret_cast<uint32_t*>(a.y + size_t(bh) * 2 * D + lane * C);
+#pragma unroll
+  for (int k = 0; k < C; k += 2) {
+    const float g0 = a.gain ? a.gain[lane * C + k] : 1.f, g1 = a.gain ? a.gain[lane * C + k + 1] : 1.f;
+    y[k / 2] = pack2<BF>(out[k] * g0, out[k + 1] * g1);
+  }
+  if (lane == 0) join_finish(a, bh, b, head);
 }
 
 }  // namespace da

@@ -25,37 +25,42 @@ struct EvictArgs {
 
 constexpr int SELECT_THREADS = 512, SELECT_WARPS = SELECT_THREADS / 32;
 constexpr int SELECT_MOST_KEYS = 48 * 1024;      // that fit in shared memory
+constexpr int SELECT_AHEAD = 8;                  // slots whose loads a thread has under way together
 
 // Order of a slot: whole numbers, larger = rather kept.  NaN counts as larger than every number, -0 as 0.
-__device__ __forceinline__ uint32_t evict_key(const EvictArgs& a, long long at, int newest_from) {
-  const int pos = a.c.positions[at];
-  const float w = a.c.weights ? a.c.weights[at] : 0.f;
+__device__ __forceinline__ uint32_t evict_key(const EvictArgs& a, int pos, float w, int newest_from) {
   if (pos >= newest_from) return 0xffffffffu;
   if (!a.c.weights) return uint32_t(max(pos, 0));
   const uint32_t u = w != w ? 0x7fc00000u : __float_as_uint(w + 0.f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ uint32_t evict_key(const EvictArgs& a, long long at, int newest_from) {
+  return evict_key(a, a.c.positions[at], a.c.weights ? a.c.weights[at] : 0.f, newest_from);
+}
 
-// sum of `x` over the threads before this one; `total`: over all.  `buf`: SELECT_WARPS ints of this call's own
-__device__ __forceinline__ int block_before(int x, int* buf, int& total) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int incl = x;
+// sums of x and y over the threads before this one, in place; `total`: of y over all.  `buf`: SELECT_WARPS places of this call's own
+__device__ __forceinline__ void block_before(int& x, int& y, int2* buf, int& total) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, x0 = x, y0 = y;
+  auto scan = [&](int& v) {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += y;
-  }
-  if (lane == 31) buf[warp] = incl;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+  };
+  scan(x);
+  scan(y);
+  if (lane == 31) buf[warp] = make_int2(x, y);
   __syncthreads();
-  int s = lane < SELECT_WARPS ? buf[lane] : 0;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, s, o);
-    if (lane >= o) s += y;
-  }
-  total = __shfl_sync(0xffffffffu, s, 31);
-  const int before = __shfl_sync(0xffffffffu, s, max(warp - 1, 0));
-  return (warp ? before : 0) + incl - x;
+  const int2 all = lane < SELECT_WARPS ? buf[lane] : make_int2(0, 0);
+  int sx = all.x, sy = all.y;
+  scan(sx);
+  scan(sy);
+  total = __shfl_sync(0xffffffffu, sy, 31);
+  sx = __shfl_sync(0xffffffffu, sx - all.x, warp);
+  sy = __shfl_sync(0xffffffffu, sy - all.y, warp);
+  x += sx - x0;
+  y += sy - y0;
 }
 
 // A list of moves, by one block of `blocks`; all its threads call it.  Thread: one 16-byte piece of a row, UNROLL rows under way together.
@@ -79,8 +84,10 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, MovePlaces<D, THRE
         const long long base = (long long)bh * c.slots;
         const int pos = c.positions[base + mv.x];
         const float w = c.weights ? c.weights[base + mv.x] : 0.f;
-        place_row(c, places.from, threadIdx.x, b, head, mv.x);
-        place_row(c, places.to, threadIdx.x, b, head, mv.y);
+        const int ef = cache_page(c, mv.x), et = cache_page(c, mv.y);
+        const int idf = cache_page_load(c, b, ef), idt = cache_page_load(c, b, et);
+        place_row(c, places.from, threadIdx.x, b, head, mv.x, ef, idf);
+        place_row(c, places.to, threadIdx.x, b, head, mv.y, et, idt);
         if (places.to.k[threadIdx.x] < 0) places.from.k[threadIdx.x] = -1;
         c.positions[base + mv.y] = pos;
         if (c.weights) c.weights[base + mv.y] = w;
@@ -101,9 +108,10 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, MovePlaces<D, THRE
 constexpr int SELECT_LIST = 512;                 // moves that the selection keeps in shared memory
 
 template <int D>
-__global__ void __launch_bounds__(SELECT_THREADS) diffattn_cache_select_kernel(const EvictArgs a) {
+__global__ void __launch_bounds__(SELECT_THREADS, 4) diffattn_cache_select_kernel(const EvictArgs a) {
   extern __shared__ uint32_t keys[];
-  __shared__ int hist[4][256], buf[2][SELECT_WARPS];
+  __shared__ int hist[4][256];
+  __shared__ int2 buf[2][SELECT_WARPS];
   __shared__ int2 near_list[SELECT_LIST];
   __shared__ MovePlaces<D, SELECT_THREADS> places;
   const CacheArgs& c = a.c;
@@ -120,11 +128,23 @@ __global__ void __launch_bounds__(SELECT_THREADS) diffattn_cache_select_kernel(c
   const long long base = (long long)bh * c.slots;
   // the keep-th largest key, eight bits at a time: how many keys that agree with the bits so far have each next digit
   auto key = [&](int i) { return a.cached_keys ? keys[i] : evict_key(a, base + i, newest_from); };
-#pragma unroll 4
-  for (int i = tid; i < len; i += SELECT_THREADS) {
-    const uint32_t k = evict_key(a, base + i, newest_from);
-    if (a.cached_keys) keys[i] = k;
-    atomicAdd(&hist[0][k >> 24], 1);
+  for (int i0 = tid; i0 < len; i0 += SELECT_THREADS * SELECT_AHEAD) {
+    int pos[SELECT_AHEAD];
+    float w[SELECT_AHEAD];
+#pragma unroll
+    for (int x = 0; x < SELECT_AHEAD; ++x) {
+      const int i = min(i0 + x * SELECT_THREADS, len - 1);
+      pos[x] = c.positions[base + i];
+      w[x] = c.weights ? c.weights[base + i] : 0.f;
+    }
+#pragma unroll
+    for (int x = 0; x < SELECT_AHEAD; ++x) {
+      const int i = i0 + x * SELECT_THREADS;
+      if (i >= len) break;
+      const uint32_t k = evict_key(a, pos[x], w[x], newest_from);
+      if (a.cached_keys) keys[i] = k;
+      atomicAdd(&hist[0][k >> 24], 1);
+    }
   }
   uint32_t prefix = 0;
   int want = a.keep, alike = 0;      // of the `alike` keys that agree with `prefix`, `want` stay
@@ -171,9 +191,9 @@ __global__ void __launch_bounds__(SELECT_THREADS) diffattn_cache_select_kernel(c
   const int i0 = min(tid * run, len), i1 = min(i0 + run, len);
   int rank = 0, total;
   if (alike != want) {               // (all 32 bits of `prefix` are known)
-    int n = 0;
-    for (int i = i0; i < i1; ++i) n += key(i) == prefix;
-    rank = block_before(n, buf[0], total);
+    int none = 0;
+    for (int i = i0; i < i1; ++i) rank += key(i) == prefix;
+    block_before(rank, none, buf[0], total);
   }
   auto stays = [&](uint32_t k, int& r) {
     if (alike == want) return k >= prefix;
@@ -187,10 +207,8 @@ __global__ void __launch_bounds__(SELECT_THREADS) diffattn_cache_select_kernel(c
     holes += !kept && i < a.keep;
   }
   int2* list = a.most <= SELECT_LIST ? near_list : a.moves + (long long)bh * a.most;
-  const int holes_before = block_before(holes, buf[1], total);
-  __syncthreads();
-  int at = block_before(moves, buf[1], total);
-  int to = holes_before;
+  block_before(holes, moves, buf[1], total);
+  int at = moves, to = holes;
   r = rank;
   for (int i = i0; i < i1; ++i) {
     const bool kept = stays(key(i), r);

@@ -34,7 +34,7 @@ AttendSpace attend_space(const DiffAttnCacheParams* p) {
   const uint64_t pieces = uint64_t(attend_workers(p)) + uint64_t(p->B) * p->H;
   uint64_t at = 0;
   auto take = [&](uint64_t& where, uint64_t bytes) { where = at; at += round256(bytes); };
-  take(s.prefix, 4 * (uint64_t(p->B) + 1));
+  take(s.prefix, 4 * (uint64_t(p->B) + 2));
   take(s.length, 4 * uint64_t(p->B));
   take(s.position, 4 * uint64_t(p->B));
   take(s.stats, 16 * pieces);
@@ -152,14 +152,15 @@ int attend_launch(const DiffAttnCacheParams* p, da::AttendArgs& a) {
   const cudaStream_t stream = static_cast<cudaStream_t>(p->stream);
   const int sms = sm_count(p->device);
   if ((rc = launch(kernel, dim3(sms), da::attend::Geo<D>::THREADS, smem, stream, false, k1, k2, v, a))) return rc;
-  // 1024 threads for more than a dozen pieces a (sequence, head): B1 H16 N16384 D64 (74 pieces) XX us instead of XX
+  // How many pieces a (sequence, head) has goes by how many of them share the workers, and by its tiles.
   const int bh = p->B * p->H;
-  if (a.workers > 12 * bh) {
-    a.join_blocks = std::min(bh, sms * 2);
-    return launch(da::diffattn_cache_join_kernel<D, 1024, BF, TRACK>, dim3(a.join_blocks + (TRACK ? bh * ((sms + bh - 1) / bh) : 0)), 1024, 0, stream, true, a);
-  }
-  a.join_blocks = std::min(bh, sms * 8);
-  return launch(da::diffattn_cache_join_kernel<D, 256, BF, TRACK>, dim3(a.join_blocks + (TRACK ? bh * ((4 * sms + bh - 1) / bh) : 0)), 256, 0, stream, true, a);
+  const long long pieces = std::min((long long)a.workers / bh, most_tiles(p));
+  auto weights = [&](int blocks) { return TRACK ? bh * ((blocks + bh - 1) / bh) : 0; };
+  a.join_blocks = bh;
+  if (pieces > 12) return launch(da::diffattn_cache_join_kernel<D, 1024, BF, TRACK>, dim3(bh + weights(sms)), 1024, 0, stream, true, a);
+  if (pieces > 2) return launch(da::diffattn_cache_join_kernel<D, 256, BF, TRACK>, dim3(bh + weights(4 * sms)), 256, 0, stream, true, a);
+  a.join_blocks = (bh + da::JOIN_FEW / 32 - 1) / (da::JOIN_FEW / 32);
+  return launch(da::diffattn_cache_join_few_kernel<D, BF, TRACK>, dim3(a.join_blocks + weights(4 * sms)), da::JOIN_FEW, 0, stream, true, a);
 }
 template <int D>
 int attend_launch(const DiffAttnCacheParams* p, da::AttendArgs& a) {
