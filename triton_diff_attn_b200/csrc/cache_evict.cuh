@@ -23,7 +23,9 @@ struct EvictArgs {
   int moves_at_once;                 // the selection carries its moves out
 };
 
-constexpr int SELECT_THREADS = 512, SELECT_WARPS = SELECT_THREADS / 32;
+// (256 threads: the chain of loads and barriers counts, not the arithmetic; 512 select no faster, and fewer CTAs are resident: a step of B32 H16 N2048
+// 116 us with 512, 110 with 256)
+constexpr int SELECT_THREADS = 256, SELECT_WARPS = SELECT_THREADS / 32;
 constexpr int SELECT_MOST_KEYS = 48 * 1024;      // that fit in shared memory
 constexpr int SELECT_AHEAD = 8;                  // slots whose loads a thread has under way together
 
@@ -38,29 +40,26 @@ __device__ __forceinline__ uint32_t evict_key(const EvictArgs& a, long long at, 
   return evict_key(a, a.c.positions[at], a.c.weights ? a.c.weights[at] : 0.f, newest_from);
 }
 
-// sums of x and y over the threads before this one, in place; `total`: of y over all.  `buf`: SELECT_WARPS places of this call's own
-__device__ __forceinline__ void block_before(int& x, int& y, int2* buf, int& total) {
+// sums of x and y over the threads before this one, in place; `all`: over all of them.  `buf`: SELECT_WARPS places, free again after the next barrier
+__device__ __forceinline__ void block_before(int& x, int& y, int2* buf, int2& all) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, x0 = x, y0 = y;
-  auto scan = [&](int& v) {
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, v, o);
-      if (lane >= o) v += u;
-    }
-  };
-  scan(x);
-  scan(y);
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, x, o), v = __shfl_up_sync(0xffffffffu, y, o);
+    if (lane >= o) { x += u; y += v; }
+  }
   if (lane == 31) buf[warp] = make_int2(x, y);
   __syncthreads();
-  const int2 all = lane < SELECT_WARPS ? buf[lane] : make_int2(0, 0);
-  int sx = all.x, sy = all.y;
-  scan(sx);
-  scan(sy);
-  total = __shfl_sync(0xffffffffu, sy, 31);
-  sx = __shfl_sync(0xffffffffu, sx - all.x, warp);
-  sy = __shfl_sync(0xffffffffu, sy - all.y, warp);
-  x += sx - x0;
-  y += sy - y0;
+  x -= x0;
+  y -= y0;
+  all = make_int2(0, 0);
+#pragma unroll
+  for (int w = 0; w < SELECT_WARPS; ++w) {
+    const int2 v = buf[w];
+    if (w < warp) { x += v.x; y += v.y; }
+    all.x += v.x;
+    all.y += v.y;
+  }
 }
 
 // A list of moves, by one block of `blocks`; all its threads call it.  Thread: one 16-byte piece of a row, UNROLL rows under way together.
@@ -108,7 +107,7 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, MovePlaces<D, THRE
 constexpr int SELECT_LIST = 512;                 // moves that the selection keeps in shared memory
 
 template <int D>
-__global__ void __launch_bounds__(SELECT_THREADS, 4) diffattn_cache_select_kernel(const EvictArgs a) {
+__global__ void __launch_bounds__(SELECT_THREADS) diffattn_cache_select_kernel(const EvictArgs a) {
   extern __shared__ uint32_t keys[];
   __shared__ int hist[4][256];
   __shared__ int2 buf[2][SELECT_WARPS];
@@ -185,36 +184,44 @@ __global__ void __launch_bounds__(SELECT_THREADS, 4) diffattn_cache_select_kerne
     alike = __shfl_sync(0xffffffffu, size, owner);
     if (alike == want) break;        // all of them stay: whatever their lower bits are
   }
-  // Keys above `prefix` stay, and of those that agree with it the first `want`.  Survivors behind `keep` and holes below it in slot order: a
-  // thread has a run of slots (an odd number, so that a warp's reads fall into different banks)
-  const int run = ((len + SELECT_THREADS - 1) / SELECT_THREADS) | 1;
-  const int i0 = min(tid * run, len), i1 = min(i0 + run, len);
-  int rank = 0, total;
-  if (alike != want) {               // (all 32 bits of `prefix` are known)
-    int none = 0;
-    for (int i = i0; i < i1; ++i) rank += key(i) == prefix;
-    block_before(rank, none, buf[0], total);
-  }
-  auto stays = [&](uint32_t k, int& r) {
-    if (alike == want) return k >= prefix;
-    if (k != prefix) return k > prefix;
-    return r++ < want;
-  };
-  int moves = 0, holes = 0, r = rank;
-  for (int i = i0; i < i1; ++i) {
-    const bool kept = stays(key(i), r);
-    moves += kept && i >= a.keep;
-    holes += !kept && i < a.keep;
-  }
+  // Keys above `prefix` stay, and of those that agree with it the first `want`.  Survivors behind `keep` and holes below it in slot order: a thread
+  // has a run of at most 31 neighbours (an odd number, so that a warp's reads fall into different banks) and keeps in a mask which of them
+  // are one or the other.
+  const bool ties = alike != want;   // (then all 32 bits of `prefix` are known)
   int2* list = a.most <= SELECT_LIST ? near_list : a.moves + (long long)bh * a.most;
-  block_before(holes, moves, buf[1], total);
-  int at = moves, to = holes;
-  r = rank;
-  for (int i = i0; i < i1; ++i) {
-    const bool kept = stays(key(i), r);
-    if (kept && i >= a.keep) list[at++].x = i;
-    if (!kept && i < a.keep) list[to++].y = i;
+  int equal = 0, holes = 0, moves = 0;           // before the current round
+  for (int c0 = 0; c0 < len; c0 += 31 * SELECT_THREADS) {
+    const int left = min(len - c0, 31 * SELECT_THREADS), run = min((left + SELECT_THREADS - 1) / SELECT_THREADS | 1, 31);
+    const int i0 = min(c0 + tid * run, c0 + left), i1 = min(i0 + run, c0 + left);
+    uint32_t same = 0, kept = 0;
+    for (int i = i0; i < i1; ++i) {
+      const uint32_t k = key(i);
+      kept |= uint32_t(k >= prefix) << (i - i0);
+      same |= uint32_t(k == prefix) << (i - i0);
+    }
+    int2 all;
+    if (ties) {
+      int rank = __popc(same), none = 0;
+      block_before(rank, none, buf[0], all);
+      rank += equal;
+      for (uint32_t m = same; m; m &= m - 1)      // those behind the first `want` go
+        if (rank++ >= want) kept &= ~(m & -m);
+      equal += all.x;
+    }
+    const int low = min(max(a.keep - i0, 0), i1 - i0);      // slots of the run below `keep`
+    const uint32_t mask_low = low >= 32 ? 0xffffffffu : (1u << low) - 1;
+    uint32_t hole = ~kept & mask_low, moved = kept & ~mask_low;
+    int x = __popc(hole), y = __popc(moved);
+    block_before(x, y, buf[1], all);
+    x += holes;
+    y += moves;
+    for (; hole; hole &= hole - 1) list[x++].y = i0 + __ffs(hole) - 1;
+    for (; moved; moved &= moved - 1) list[y++].x = i0 + __ffs(moved) - 1;
+    holes += all.x;
+    moves += all.y;
+    if (c0 + 31 * SELECT_THREADS < len) __syncthreads();      // (the next round writes buf)
   }
+  int total = moves;
   __syncthreads();
   if (a.moves_at_once) {
     move_rows<D, SELECT_THREADS>(a, places, bh, list, total, 0, 1);
