@@ -104,7 +104,12 @@ def tile_shape(d, page):
     r = t
     while page % r:
         r //= 2
-    return (t, r, 0) if r >= 8 else (t, t, -(-page // t))
+    per_page = -(-page // t)
+    if r >= 8:
+        return t, r, 0
+    if 10 * per_page * t <= page * {4: 13, 2: 15, 1: 20}[r] or r * (64 if d == 32 else 128) < 128:
+        return t, t, per_page
+    return t, r, 0
 
 
 def tiles_of(n, page, shape, token):
@@ -131,7 +136,7 @@ def test_tiles_cover_every_token_once(d):
     for page in list(range(1, 40)) + [48, 64, 100, 128, 1000]:
         shape = tile_shape(d, page)
         t, box, per_page = shape
-        assert t % box == 0 and box % 8 == 0           # whole periods of the swizzle
+        assert t % box == 0 and box * (64 if d == 32 else 128) % 128 == 0 and (per_page or page % box == 0)
         for n in list(range(0, 3 * t + 2)) + [page - 1, page, page + 1, 4 * page, 4 * page + 1]:
             for token in (0, 1):
                 m, seen = tiles_of(n, page, shape, token), []

@@ -103,7 +103,7 @@ LENGTHS = {   # by head dim: around a tile's 1024 / D tokens
 
 
 @pytest.mark.parametrize("d", [32, 64, 128])
-@pytest.mark.parametrize("page", [1, 2, 7, 8, 16, 24, 64, 100])
+@pytest.mark.parametrize("page", [1, 2, 4, 7, 8, 16, 24, 33, 64, 100])
 @pytest.mark.parametrize("form", ["plain", "track", "token", "token_track"])
 def test_attend_pages_and_lengths(pkg, d, page, form):
     dt = torch.bfloat16 if (page + d // 32) % 2 else torch.float16

@@ -3,17 +3,22 @@
 
 namespace {
 
-// How a tile of T rows is fetched.  Where page size and tile have a common divisor of 8 or more (every page size that is a multiple of 8), tiles
-// run on over the pages in boxes of that many rows, each inside one page and, in shared memory, at a whole period of the swizzle.
-// Else a tile stays inside its page and its last one is not full (a page of 100 slots: 7 tiles of 16; a page of 1: a tile for every token).
+// How a tile of T rows is fetched: it runs on over the pages in boxes of r rows, r the common divisor of page size and T, each inside one page; or it
+// stays inside its page, whose last tile is then not full.  Eight or more rows to a box cost nothing.  Fewer cost more requests: B8 H16
+// N2048 D64 takes 29 us with pages of 8, 32 with 4, 55 with 1.  So tiles stay inside their pages where that wastes less, by these factors (D =
+// 32 / 128, pages of 100: 33 / 32 us against 36 / 38).  A box's rows have to fill 128 bytes of shared memory; where they lie in the swizzle's
+// pattern goes by their address.
 struct TileShape { int rows, box_rows, tiles_per_page; };
 int tile_rows(int D) { return D == 32 ? da::attend::Geo<32>::T : D == 64 ? da::attend::Geo<64>::T : da::attend::Geo<128>::T; }
 TileShape tile_shape(const DiffAttnCacheParams* p) {
-  const int T = tile_rows(p->D);
+  const int T = tile_rows(p->D), row_bytes = p->D == 32 ? 64 : 128;
   int r = T;
   while (p->page_size % r) r /= 2;             // (T is a power of two)
   if (r >= 8) return {T, r, 0};
-  return {T, T, (p->page_size + T - 1) / T};
+  const int per_page = (p->page_size - 1) / T + 1;
+  const bool fits = 10ll * per_page * T <= (long long)p->page_size * (r == 4 ? 13 : r == 2 ? 15 : 20);
+  if (fits || r * row_bytes < 128) return {T, T, per_page};
+  return {T, r, 0};
 }
 // tiles of a full sequence
 long long most_tiles(const DiffAttnCacheParams* p) {
@@ -157,7 +162,7 @@ int attend_launch(const DiffAttnCacheParams* p, da::AttendArgs& a) {
   const long long pieces = std::min((long long)a.workers / bh, most_tiles(p));
   auto weights = [&](int blocks) { return TRACK ? bh * ((blocks + bh - 1) / bh) : 0; };
   a.join_blocks = bh;
-  if (pieces > 12) return launch(da::diffattn_cache_join_kernel<D, 1024, BF, TRACK>, dim3(bh + weights(sms)), 1024, 0, stream, true, a);
+  if (pieces > 40) return launch(da::diffattn_cache_join_kernel<D, 1024, BF, TRACK>, dim3(bh + weights(sms)), 1024, 0, stream, true, a);
   if (pieces > 2) return launch(da::diffattn_cache_join_kernel<D, 256, BF, TRACK>, dim3(bh + weights(4 * sms)), 256, 0, stream, true, a);
   a.join_blocks = (bh + da::JOIN_FEW / 32 - 1) / (da::JOIN_FEW / 32);
   return launch(da::diffattn_cache_join_few_kernel<D, BF, TRACK>, dim3(a.join_blocks + weights(4 * sms)), da::JOIN_FEW, 0, stream, true, a);
