@@ -41,6 +41,8 @@ BAD = [
     (ALL, "page_table", 0, -1), (ALL, "lengths", 0, -1), (ALL, "v_pages", 0x10008, -6), (ALL, "kp_stride_head", 60, -5), (ALL, "kp_stride_page", 0, -5),
     (ALL, "vp_stride_slot", 64, -5), (ALL, "table_stride", 3, -5), (ALL, "positions", 0, -1), (ALL, "device", 64, -3), (ALL, "device", -1, -3),
     (("append",), "T", -1, -3), (("append", "attend"), "k2", 0, -1), (("append", "attend"), "v", 0x10008, -6), (("append", "attend"), "v_stride_h", 12, -5),
+    (("append",), "T", 2 ** 31 - 1, -3), (("append",), "counts", 0x10002, -6), (ALL, "lengths", 0x10002, -6), (ALL, "page_table", 0x10001, -6),
+    (ALL, "weights", 0x10002, -6), (("attend",), "y", 0x10002, -6), (("attend",), "gain", 0x10002, -6), (("attend",), "lambda_scale", 0x10002, -6),
     (("append",), "k_stride_t", 0, -5), (("attend",), "q1", 0, -1), (("attend",), "q2", 0x10004, -6), (("attend",), "q_stride_h", 4, -5),
     (("attend",), "lambda_dtype", 9, -7), (("attend",), "y", 0, -1), (("attend",), "lambda_scale", 0, -1),
     (("evict",), "keep", 0, -3), (("evict",), "keep", 65, -3), (("evict",), "recent", 9, -3), (("evict",), "recent", -1, -3),

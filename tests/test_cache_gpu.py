@@ -398,6 +398,46 @@ def test_capture_streams_and_threads(pkg):
     pkg.device_status(0)
 
 
+def test_two_graphs_at_once(pkg):
+    """Queries that write nothing may overlap: two captured calls on one cache, replayed on two streams, have workspaces of their own."""
+    c = make(pkg, [900, 0, 333, 1500], 4, 64, 16, seed=12)
+    lam = torch.tensor([0.5], device=DEV)
+    qs = [queries(4, 4, 64, torch.float16, seed=s) for s in (1, 2)]
+    want = [c.attend(q[0], q[1], lam) for q in qs]
+    graphs, ys = [], []
+    for q in qs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            ys.append(c.attend(q[0], q[1], lam))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in qs]
+    for _ in range(20):
+        for st, g in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, w) for y, w in zip(ys, want))
+
+
+def test_attend_many_sequences(pkg):
+    """The largest batch, most of it not in use."""
+    lengths = [0] * 4096
+    for i in (0, 1, 31, 32, 255, 256, 2048, 4094, 4095):
+        lengths[i] = 1 + i % 50
+    c = make(pkg, lengths, 1, 32, 64, seed=13)
+    q1, q2, *_ = queries(4096, 1, 32, torch.float16, seed=13)
+    y = c.attend(q1, q2, torch.tensor([0.5], device=DEV))
+    used = [i for i, n in enumerate(lengths) if n]
+    sub = type("C", (), dict(k1_pages=c.k1_pages, k2_pages=c.k2_pages, v_pages=c.v_pages, page_table=c.page_table[used], weights=None))
+    check_attend(sub, {"weights": None}, y[used], q1[used], q2[used], 0.5, [lengths[i] for i in used], rms=False)
+    rest = torch.ones(4096, dtype=torch.bool, device=DEV)
+    rest[used] = False
+    assert not bool(y[rest].any())
+    with pytest.raises(ValueError):
+        pkg.DiffAttnCache(4097, 1, 32, 8, device=DEV).attend(*(torch.zeros(4097, 1, 1, 32, dtype=torch.float16, device=DEV),) * 2, torch.tensor([0.5], device=DEV))
+    pkg.device_status(0)
+
+
 @pytest.mark.parametrize("d,dt", [(64, torch.float16), (128, torch.bfloat16), (32, torch.float16)])
 def test_prompt_then_generation(pkg, d, dt):
     """A layer core's prompt through its causal forward, its tokens into the cache, then token by token: every step is the last row of the causal

@@ -45,12 +45,14 @@ struct AttendArgs {
 };
 
 namespace attend {
-constexpr int MAX_B = 4096;                    // the prefix sums of all sequences lie in shared memory
+constexpr int MAX_B = 4096;                    // the prefix sums and lengths of all sequences lie in shared memory
 template <int D>
 struct Geo {
   static constexpr int T = D == 32 ? 32 : 16;  // tokens per tile: 8 KB of K1, K2, V (D = 128: 16 KB)
   static constexpr int WARPS = D == 128 ? 4 : 8, THREADS = WARPS * 32;
-  static constexpr int SLOTS = 2;              // tiles in flight per warp
+  // Tiles in flight per warp: 128 KB of requests an SM.  Three are slower (B64 H16 ragged to 4096 D64: 206 us, two 190): the SMs get their share of
+  // HBM less evenly, and the last one counts.  One, with 12 warps: 183 there, but 33 instead of 31 at B1 H16 N16384.  Six warps: 207.
+  static constexpr int SLOTS = 2;
   // a tile in shared memory: boxes of T rows of 128 bytes (K at D = 32: 64 bytes), swizzled by the engine: K1, K2, V
   static constexpr int K_ROW = D == 32 ? 64 : 128, K_BOXES = D == 128 ? 2 : 1, V_BOXES = D / 32;
   static constexpr int K_BYTES = T * D * 2, V_BYTES = 2 * K_BYTES, SLOT_BYTES = 2 * K_BYTES + V_BYTES;
@@ -59,8 +61,8 @@ struct Geo {
   static constexpr int OFF_BAR = OFF_Q + WARPS * SLOTS * Q_BYTES;
   static constexpr int OFF_SUM = OFF_BAR + WARPS * SLOTS * 8 + 16;
   static constexpr int OFF_PREFIX = OFF_SUM + WARPS * 4;
-  static constexpr int SMEM = OFF_PREFIX + 4 + 1024;      // + 4 b bytes of prefix sums; 1024 to align the ring
-  static_assert(SMEM + 4 * MAX_B <= 227 * 1024, "shared memory");
+  static constexpr int SMEM = OFF_PREFIX + 4 + 1024;      // + 8 b bytes of prefix sums and lengths; 1024 to align the ring
+  static_assert(SMEM + 8 * MAX_B <= 227 * 1024, "shared memory");
 };
 }  // namespace attend
 
@@ -174,6 +176,7 @@ diffattn_cache_attend_kernel(const __grid_constant__ CUtensorMap tm_k1, const __
   volatile int* drain_flag = abort_flag + 1;
   int* part_sum = reinterpret_cast<int*>(smem + G::OFF_SUM);
   int* prefix = reinterpret_cast<int*>(smem + G::OFF_PREFIX);
+  int* length = prefix + a.c.b + 1;            // (read once: all that follows has to agree on it)
 
   if (lane == 0) {
     for (int i = 0; i < SLOTS; ++i) mbar_init(&full[i], 1);
@@ -194,6 +197,7 @@ diffattn_cache_attend_kernel(const __grid_constant__ CUtensorMap tm_k1, const __
     const int len = cache_length(a.c, b);
     sum += attend_tiles<T>(a, len);
     prefix[b + 1] = sum;
+    length[b] = len;
     if (blockIdx.x == 0) {                     // for the joining kernel, which finds the lengths moved on
       a.length[b] = len;
       if (a.nk1 && a.c.next_position) a.position[b] = a.c.next_position[b];
@@ -228,12 +232,8 @@ diffattn_cache_attend_kernel(const __grid_constant__ CUtensorMap tm_k1, const __
   const int count = int(stretch_begin(units, workers, worker + 1) - first);
 
   // ---- loads.  Lane i fetches box i of a tile; its page is looked up one request ahead.
-  TileWalk ahead = walk_at(a, prefix, a.c.lengths, first);
-  ahead.len = min(max(ahead.len, 0), a.c.slots);
-  auto next = [&](TileWalk& w) {
-    walk_next(a, prefix, a.c.lengths, w);
-    w.len = min(max(w.len, 0), a.c.slots);
-  };
+  TileWalk ahead = walk_at(a, prefix, length, first);
+  auto next = [&](TileWalk& w) { walk_next(a, prefix, length, w); };
   struct Box { int page, in_page; };           // page -1: the engine fills the box with zeros; in_page -1: no such box
   auto look_up = [&](const TileWalk& w) {
     int slot, valid;

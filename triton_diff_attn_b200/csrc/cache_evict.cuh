@@ -215,13 +215,14 @@ __global__ void __launch_bounds__(SELECT_THREADS) diffattn_cache_select_kernel(c
     block_before(x, y, buf[1], all);
     x += holes;
     y += moves;
-    for (; hole; hole &= hole - 1) list[x++].y = i0 + __ffs(hole) - 1;
-    for (; moved; moved &= moved - 1) list[y++].x = i0 + __ffs(moved) - 1;
+    // (as many survivors as holes, and no more than `most`, as long as nobody writes positions or weights meanwhile)
+    for (; hole && x < a.most; hole &= hole - 1) list[x++].y = i0 + __ffs(hole) - 1;
+    for (; moved && y < a.most; moved &= moved - 1) list[y++].x = i0 + __ffs(moved) - 1;
     holes += all.x;
     moves += all.y;
     if (c0 + 31 * SELECT_THREADS < len) __syncthreads();      // (the next round writes buf)
   }
-  int total = moves;
+  int total = min(min(holes, moves), a.most);
   __syncthreads();
   if (a.moves_at_once) {
     move_rows<D, SELECT_THREADS>(a, places, bh, list, total, 0, 1);

@@ -50,6 +50,7 @@ AttendSpace attend_space(const DiffAttnCacheParams* p) {
 }
 int evict_most(const DiffAttnCacheParams* p) { return std::min(p->keep, p->max_pages * p->page_size - p->keep); }
 
+bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 bool good_stride(int64_t s, bool used) { return !used || (s > 0 && s % 8 == 0); }
 
 // sizes alone, for the workspace query too
@@ -63,7 +64,9 @@ int check_cache_sizes(const DiffAttnCacheParams* p) {
     return fail(DIFFATTN_ERR_BAD_SHAPE, "B=%d H=%d: B <= %d and B*H <= 65535", p->B, p->H, da::attend::MAX_B);
   if (p->page_size <= 0 || p->num_pages <= 0 || p->max_pages <= 0)
     return fail(DIFFATTN_ERR_BAD_SHAPE, "page_size=%d num_pages=%d max_pages=%d must be positive", p->page_size, p->num_pages, p->max_pages);
-  if (((long long)p->max_pages + 1) * p->page_size > INT32_MAX || most_tiles(p) * std::max(p->B, 1) > INT32_MAX)
+  // (the kernels add a page or two tiles to a slot in 32 bits)
+  if ((long long)p->max_pages * p->page_size + std::max(p->page_size, 64) > INT32_MAX || most_tiles(p) * std::max(p->B, 1) > INT32_MAX ||
+      most_tiles(p) * std::max(p->B, 1) * std::max(p->H, 1) > (1ll << 39))
     return fail(DIFFATTN_ERR_BAD_SHAPE, "max_pages=%d of %d slots: too long", p->max_pages, p->page_size);
   return DIFFATTN_OK;
 }
@@ -80,6 +83,9 @@ int check_cache(const DiffAttnCacheParams* p) {
     if (!ptrs[i]) return fail(DIFFATTN_ERR_NULL_PTR, "%s is NULL", names[i]);
   for (int i = 0; i < 3; ++i)
     if (!aligned16(ptrs[i])) return fail(DIFFATTN_ERR_MISALIGNED, "%s is not 16-byte aligned", names[i]);
+  const void* words[] = {p->page_table, p->lengths, p->next_position, p->positions, p->weights};
+  for (const void* w : words)
+    if (!aligned_to(w, 4)) return fail(DIFFATTN_ERR_MISALIGNED, "page_table, lengths, next_position, positions and weights must be 4-byte aligned");
   if ((p->positions != nullptr) != (p->next_position != nullptr)) return fail(DIFFATTN_ERR_NULL_PTR, "positions and next_position go together");
   const int64_t st[] = {p->kp_stride_page, p->kp_stride_head, p->kp_stride_slot, p->vp_stride_page, p->vp_stride_head, p->vp_stride_slot};
   const bool used[] = {p->num_pages > 1, p->H > 1, p->page_size > 1, p->num_pages > 1, p->H > 1, p->page_size > 1};
@@ -151,8 +157,8 @@ int attend_launch(const DiffAttnCacheParams* p, da::AttendArgs& a) {
   if ((rc = map(&k2, p->k2_pages, D, p->kp_stride_page, p->kp_stride_head, p->kp_stride_slot, "k2_pages"))) return rc;
   if ((rc = map(&v, p->v_pages, 2 * D, p->vp_stride_page, p->vp_stride_head, p->vp_stride_slot, "v_pages"))) return rc;
   auto kernel = da::diffattn_cache_attend_kernel<D, BF, TRACK>;
-  constexpr int most = da::attend::Geo<D>::SMEM + 4 * da::attend::MAX_B;
-  const int smem = da::attend::Geo<D>::SMEM + 4 * p->B;
+  constexpr int most = da::attend::Geo<D>::SMEM + 8 * da::attend::MAX_B;
+  const int smem = da::attend::Geo<D>::SMEM + 8 * p->B;
   if ((rc = set_smem(kernel, most, p->device))) return rc;
   const cudaStream_t stream = static_cast<cudaStream_t>(p->stream);
   const int sms = sm_count(p->device);
@@ -207,9 +213,10 @@ uint64_t diffattn_cache_workspace_bytes(const DiffAttnCacheParams* p, int32_t op
 int diffattn_cache_append(const DiffAttnCacheParams* p) {
   int rc = check_cache(p);
   if (rc) return rc < 0 ? rc : DIFFATTN_OK;
-  if (p->T < 0) return fail(DIFFATTN_ERR_BAD_SHAPE, "T=%d", p->T);
+  if (p->T < 0 || p->T > INT32_MAX - 1024) return fail(DIFFATTN_ERR_BAD_SHAPE, "T=%d", p->T);
   if (p->T == 0) return DIFFATTN_OK;
   if ((rc = check_tokens(p, true))) return rc;
+  if (!aligned_to(p->counts, 4)) return fail(DIFFATTN_ERR_MISALIGNED, "counts is not 4-byte aligned");
   DeviceGuard guard;
   if ((rc = guard.enter(p->device))) return rc;
   if ((rc = cache_on_device(p))) return rc;
@@ -238,11 +245,13 @@ int diffattn_cache_attend(const DiffAttnCacheParams* p) {
   const char* names[] = {"q1", "q2", "lambda_scale", "y"};
   for (int i = 0; i < 4; ++i)
     if (!ptrs[i]) return fail(DIFFATTN_ERR_NULL_PTR, "%s is NULL", names[i]);
-  if (!aligned16(p->q1) || !aligned16(p->q2)) return fail(DIFFATTN_ERR_MISALIGNED, "q1/q2 not 16-byte aligned");
+  if (!aligned16(p->q1) || !aligned16(p->q2) || !aligned16(p->y)) return fail(DIFFATTN_ERR_MISALIGNED, "q1/q2/y not 16-byte aligned");
   if (!good_stride(p->q_stride_b, p->B > 1) || !good_stride(p->q_stride_h, p->H > 1))
     return fail(DIFFATTN_ERR_BAD_STRIDE, "strides of q1, q2 must be positive multiples of 8 elements");
   if (p->lambda_dtype != DIFFATTN_LAMBDA_F16 && p->lambda_dtype != DIFFATTN_LAMBDA_F32 && p->lambda_dtype != DIFFATTN_LAMBDA_BF16)
     return fail(DIFFATTN_ERR_BAD_DTYPE, "lambda_dtype %d unknown", p->lambda_dtype);
+  if (!aligned_to(p->lambda_scale, p->lambda_dtype == DIFFATTN_LAMBDA_F32 ? 4 : 2) || !aligned_to(p->gain, 4))
+    return fail(DIFFATTN_ERR_MISALIGNED, "lambda_scale or gain is not aligned to its type");
   const bool token = p->k1 || p->k2 || p->v;
   if (token && (rc = check_tokens(p, false))) return rc;
   DeviceGuard guard;
