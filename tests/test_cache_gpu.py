@@ -398,6 +398,68 @@ def test_capture_streams_and_threads(pkg):
     pkg.device_status(0)
 
 
+@pytest.mark.parametrize("captured", [False, True])
+def test_right_behind_its_inputs(pkg, captured):
+    """Kernels and copies that write queries, lengths, page table and rows right in front of a call: it reads what they wrote."""
+    h, d, page, n = 4, 64, 16, 300
+    c = make(pkg, [n, n], h, d, page, track=True, seed=14, room=40)
+    lam = torch.tensor([0.5], device=DEV)
+    q1, q2, k1, k2, v = queries(2, h, d, torch.float16, seed=14)
+    other = c.page_table.flip(0).contiguous()            # the two sequences change places: pages, rows and weights go along
+    lens = [torch.tensor(x, dtype=torch.int32, device=DEV) for x in ([n, 100], [37, n])]
+    big = torch.randn(64 << 20, device=DEV)
+    zero = torch.zeros_like(c.weights)
+
+    def calls():
+        out = []
+        for i in range(6):
+            big.mul_(1.0)                                # something long ahead, so that the call is enqueued while it runs
+            q1.mul_(-1.0)
+            c.page_table.copy_(other if i % 2 else other.flip(0))
+            c.lengths.copy_(lens[i % 2])
+            c.weights.copy_(zero)
+            c.v_pages.mul_(-1.0)
+            y = c.attend(q1, q2, lam, k1=k1, k2=k2, v=v)
+            c.append(k1, k2, v)
+            c.evict(30)
+            out += [y, c.weights.clone(), c.lengths.clone()]
+        return out
+
+    state = [t.clone() for t in (c.k1_pages, c.k2_pages, c.v_pages, c.page_table, c.lengths, c.next_position, c.positions, c.weights, q1)]
+
+    def restore():
+        for t, x in zip((c.k1_pages, c.k2_pages, c.v_pages, c.page_table, c.lengths, c.next_position, c.positions, c.weights, q1), state):
+            t.copy_(x)
+        torch.cuda.synchronize()
+
+    class Slow:                                          # the same calls with a wait behind every one of them
+        def __getattr__(self, name):
+            def call(*a, **kw):
+                torch.cuda.synchronize()
+                r = getattr(c0, name)(*a, **kw)
+                torch.cuda.synchronize()
+                return r
+            return call if name in ("attend", "append", "evict") else getattr(c0, name)
+
+    c0, c = c, Slow()
+    restore()
+    want = calls()
+    c = c0
+    restore()
+    if captured:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got = calls()
+        restore()
+        g.replay()
+    else:
+        got = calls()
+    torch.cuda.synchronize()
+    same = lambda a, b: torch.equal(a.view(torch.int16) if a.dtype == torch.float16 else a.view(torch.int32), b.view(torch.int16) if b.dtype == torch.float16 else b.view(torch.int32))
+    assert all(same(a, b) for a, b in zip(got, want))
+    pkg.device_status(0)
+
+
 def test_two_graphs_at_once(pkg):
     """Queries that write nothing may overlap: two captured calls on one cache, replayed on two streams, have workspaces of their own."""
     c = make(pkg, [900, 0, 333, 1500], 4, 64, 16, seed=12)

@@ -187,6 +187,7 @@ diffattn_cache_attend_kernel(const __grid_constant__ CUtensorMap tm_k1, const __
     *drain_flag = 0;
     tma_prefetch_desc(&tm_k1); tma_prefetch_desc(&tm_k2); tma_prefetch_desc(&tm_v);
   }
+  griddep_wait();
   griddep_launch();
 
   // ---- tiles of every sequence, summed up: a thread takes `per` consecutive sequences
@@ -542,6 +543,7 @@ __global__ void __launch_bounds__(JT) diffattn_cache_join_kernel(const __grid_co
   __shared__ float ssq[2 * D / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   griddep_wait();
+  griddep_launch();
   const int nb = a.c.b, heads = a.c.h;
   if (int(blockIdx.x) >= a.join_blocks) {
     if constexpr (TRACK) {
@@ -624,6 +626,7 @@ __global__ void __launch_bounds__(JOIN_FEW) diffattn_cache_join_few_kernel(const
   constexpr int C = 2 * D / 32;                // value columns of a lane, neighbours: 2, 4 or 8
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   griddep_wait();
+  griddep_launch();
   const int nb = a.c.b, heads = a.c.h;
   if (int(blockIdx.x) >= a.join_blocks) {
     if constexpr (TRACK) {

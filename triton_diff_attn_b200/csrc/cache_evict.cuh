@@ -114,6 +114,7 @@ __global__ void __launch_bounds__(SELECT_THREADS) diffattn_cache_select_kernel(c
   __shared__ int2 near_list[SELECT_LIST];
   __shared__ MovePlaces<D, SELECT_THREADS> places;
   const CacheArgs& c = a.c;
+  griddep_wait();
   griddep_launch();
   const int bh = blockIdx.x, b = bh / c.h, tid = threadIdx.x, lane = tid & 31;
   const int newest_from = c.next_position[b] - a.recent;
@@ -240,6 +241,7 @@ template <int D>
 __global__ void __launch_bounds__(MOVE_THREADS) diffattn_cache_move_kernel(const EvictArgs a) {
   __shared__ MovePlaces<D, MOVE_THREADS> places;
   griddep_wait();
+  griddep_launch();
   const int bh = blockIdx.y, b = bh / a.c.h;
   move_rows<D, MOVE_THREADS>(a, places, bh, a.moves + (long long)bh * a.most, a.count[bh], blockIdx.x, gridDim.x);
   if (blockIdx.x == 0 && bh == b * a.c.h && threadIdx.x == 0 && a.c.lengths[b] > a.keep) a.c.lengths[b] = a.keep;
@@ -248,6 +250,7 @@ __global__ void __launch_bounds__(MOVE_THREADS) diffattn_cache_move_kernel(const
 // The lengths alone, where the selection has moved everything.
 __global__ void __launch_bounds__(MOVE_THREADS) diffattn_cache_shorten_kernel(const EvictArgs a) {
   griddep_wait();
+  griddep_launch();
   const int b = blockIdx.x * MOVE_THREADS + threadIdx.x;
   if (b < a.c.b && a.c.lengths[b] > a.keep) a.c.lengths[b] = a.keep;
 }

@@ -162,7 +162,7 @@ int attend_launch(const DiffAttnCacheParams* p, da::AttendArgs& a) {
   if ((rc = set_smem(kernel, most, p->device))) return rc;
   const cudaStream_t stream = static_cast<cudaStream_t>(p->stream);
   const int sms = sm_count(p->device);
-  if ((rc = launch(kernel, dim3(sms), da::attend::Geo<D>::THREADS, smem, stream, false, k1, k2, v, a))) return rc;
+  if ((rc = launch(kernel, dim3(sms), da::attend::Geo<D>::THREADS, smem, stream, true, k1, k2, v, a))) return rc;
   // How many pieces a (sequence, head) has goes by how many of them share the workers, and by its tiles.
   const int bh = p->B * p->H;
   const long long pieces = std::min((long long)a.workers / bh, most_tiles(p));
@@ -186,7 +186,7 @@ int evict_launch(const DiffAttnCacheParams* p, const da::EvictArgs& a) {
   const cudaStream_t stream = static_cast<cudaStream_t>(p->stream);
   const int bh = p->B * p->H;
   if ((rc = set_smem(da::diffattn_cache_select_kernel<D>, da::SELECT_MOST_KEYS * 4, p->device))) return rc;
-  if ((rc = launch(da::diffattn_cache_select_kernel<D>, dim3(bh), da::SELECT_THREADS, a.cached_keys ? a.c.slots * 4 : 0, stream, false, a))) return rc;
+  if ((rc = launch(da::diffattn_cache_select_kernel<D>, dim3(bh), da::SELECT_THREADS, a.cached_keys ? a.c.slots * 4 : 0, stream, true, a))) return rc;
   if (a.moves_at_once)
     return launch(da::diffattn_cache_shorten_kernel, dim3((p->B + da::MOVE_THREADS - 1) / da::MOVE_THREADS), da::MOVE_THREADS, 0, stream, true, a);
   // as many CTAs as the SMs hold, spread over the (sequence, head)s, but no more than there can be moves for
@@ -234,7 +234,7 @@ int diffattn_cache_append(const DiffAttnCacheParams* p) {
   const int rows = da::APPEND_THREADS / (p->D / 2) * da::APPEND_UNROLL;
   const dim3 grid((p->T + rows - 1) / rows, p->B * p->H);
   auto kernel = p->D == 32 ? da::diffattn_cache_append_kernel<32> : p->D == 64 ? da::diffattn_cache_append_kernel<64> : da::diffattn_cache_append_kernel<128>;
-  if ((rc = launch(kernel, grid, da::APPEND_THREADS, 0, stream, false, a))) return rc;
+  if ((rc = launch(kernel, grid, da::APPEND_THREADS, 0, stream, true, a))) return rc;
   return launch(da::diffattn_cache_advance_kernel, dim3((p->B + da::APPEND_THREADS - 1) / da::APPEND_THREADS), da::APPEND_THREADS, 0, stream, true, a);
 }
 
