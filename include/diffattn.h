@@ -204,12 +204,15 @@ typedef struct DiffAttnCacheParams {
   int32_t reserved;
   void* workspace;                 /* diffattn_cache_workspace_bytes(), 256-byte aligned */
   uint64_t workspace_bytes;
+  int32_t* counter;                /* append, evict: one int32 of this cache, 0 before its first call; every call leaves it 0 */
 } DiffAttnCacheParams;
 
 enum { DIFFATTN_CACHE_APPEND = 0, DIFFATTN_CACHE_ATTEND = 1, DIFFATTN_CACHE_EVICT = 2 };
 
 /* Stores k1, k2, v behind each sequence's last token (positions follow on, weights start at 0) and moves lengths and next_position on. */
 int diffattn_cache_append(const DiffAttnCacheParams* p);
+/* Every sequence starts anew: lengths and next_position (or NULL) of B sequences become 0. */
+int diffattn_cache_reset(int32_t device, void* stream, int32_t B, int32_t* lengths, int32_t* next_position);
 /* y = (softmax(s q1 K1^T) - lambda softmax(s q2 K2^T)) V, norm and gain as diffattn_fwd, for one query per (sequence, head) over the
  * sequence's tokens; y = 0 where it has none.  With k1, k2, v (one token per sequence) that token is stored first, as append
  * does, and takes part.  weights, where given, grow by |P_1 - lambda P_2|.  Bit-reproducible on a given GPU model. */

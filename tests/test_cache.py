@@ -28,7 +28,7 @@ def _good(L, d=64):
     p.k_stride_t, p.k_stride_h, p.k_stride_b = d, 5 * d, 15 * d
     p.v_stride_t, p.v_stride_h, p.v_stride_b = 2 * d, 10 * d, 30 * d
     p.q_stride_h, p.q_stride_b, p.table_stride = d, 3 * d, 4
-    for f in ("k1_pages", "k2_pages", "v_pages", "page_table", "lengths", "next_position", "positions", "k1", "k2", "v", "q1", "q2", "lambda_scale", "y", "workspace"):
+    for f in ("k1_pages", "k2_pages", "v_pages", "page_table", "lengths", "next_position", "positions", "k1", "k2", "v", "q1", "q2", "lambda_scale", "y", "workspace", "counter"):
         setattr(p, f, 0x10000)          # never dereferenced: every check below fails before a launch
     p.lambda_dtype, p.keep, p.recent, p.workspace_bytes = 1, 8, 2, 1 << 40
     return p
@@ -41,7 +41,7 @@ BAD = [
     (ALL, "page_table", 0, -1), (ALL, "lengths", 0, -1), (ALL, "v_pages", 0x10008, -6), (ALL, "kp_stride_head", 60, -5), (ALL, "kp_stride_page", 0, -5),
     (ALL, "vp_stride_slot", 64, -5), (ALL, "table_stride", 3, -5), (ALL, "positions", 0, -1), (ALL, "device", 64, -3), (ALL, "device", -1, -3),
     (("append",), "T", -1, -3), (("append", "attend"), "k2", 0, -1), (("append", "attend"), "v", 0x10008, -6), (("append", "attend"), "v_stride_h", 12, -5),
-    (("append",), "T", 2 ** 31 - 1, -3), (("append",), "counts", 0x10002, -6), (ALL, "lengths", 0x10002, -6), (ALL, "page_table", 0x10001, -6),
+    (("append", "evict"), "counter", 0, -1), (ALL, "counter", 0x10002, -6), (("append",), "T", 2 ** 31 - 1, -3), (("append",), "counts", 0x10002, -6), (ALL, "lengths", 0x10002, -6), (ALL, "page_table", 0x10001, -6),
     (ALL, "weights", 0x10002, -6), (("attend",), "y", 0x10002, -6), (("attend",), "gain", 0x10002, -6), (("attend",), "lambda_scale", 0x10002, -6),
     (("append",), "k_stride_t", 0, -5), (("attend",), "q1", 0, -1), (("attend",), "q2", 0x10004, -6), (("attend",), "q_stride_h", 4, -5),
     (("attend",), "lambda_dtype", 9, -7), (("attend",), "y", 0, -1), (("attend",), "lambda_scale", 0, -1),
@@ -67,12 +67,17 @@ def test_empty_and_workspace_sizes(L):
     p = _good(L)
     size = lambda op: L.lib.diffattn_cache_workspace_bytes(p, op)
     assert size(L.CACHE_APPEND) == 0 and size(7) == 0
-    assert size(L.CACHE_EVICT) == 256 + -(-8 * 6 * 8 // 256) * 256
+    assert size(L.CACHE_EVICT) == 0                       # few moves: the selecting kernel keeps them
     plain = size(L.CACHE_ATTEND)
     p.weights = 0x10000
     assert size(L.CACHE_ATTEND) - plain == 5 * 6 * 2 * 16 * 4      # four tiles of 16 tokens and the new token's, two scores each
+    p.max_pages, p.keep = 64, 500                         # 500 of 1024 slots: a list of moves, counts of them
+    assert size(L.CACHE_EVICT) == 256 + -(-8 * 6 * 500 // 256) * 256
     p.keep = 0
     assert size(L.CACHE_EVICT) == 0
+    assert L.lib.diffattn_cache_reset(0, None, 0, None, None) == 0
+    assert L.lib.diffattn_cache_reset(0, None, -1, 0x10000, None) == -3 and L.lib.diffattn_cache_reset(0, None, 2, None, None) == -1
+    assert L.lib.diffattn_cache_reset(0, None, 2, 0x10002, None) == -6 and L.lib.diffattn_cache_reset(64, None, 2, 0x10000, None) == -3
 
 
 def test_struct_matches_the_header(L, tmp_path):

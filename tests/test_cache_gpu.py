@@ -255,6 +255,29 @@ def test_append(pkg, d, dt, page, slot_major, counts):
         assert torch.equal(a, w)
 
 
+def test_append_large(pkg):
+    """As many rows as have the lengths moved on by a kernel of their own."""
+    b, h, t, d = 4, 16, 700, 64
+    c = make(pkg, [0, 30, 700, 9], h, d, 16, track=True, room=t, seed=3)
+    g = torch.Generator(device=DEV); g.manual_seed(5)
+    k1, k2, v = (torch.randn((b, h, t, w), generator=g, device=DEV).half() for w in (d, d, 2 * d))
+    for counts in (None, [700, 0, 333, 1]):
+        gets = counts or [t] * b
+        c.lengths.copy_(torch.tensor([0, 30, 700, 9], dtype=torch.int32)); c.next_position.copy_(c.lengths)
+        for p in (c.k1_pages, c.k2_pages, c.v_pages):
+            p.fill_(math.nan)
+        c.append(k1, k2, v, None if counts is None else torch.tensor(counts, device=DEV))
+        pkg.device_status(0)
+        for i, (n, m) in enumerate(zip([0, 30, 700, 9], gets)):
+            at = torch.arange(n, n + m, device=DEV)
+            pages = c.page_table[i].long()[at // 16]
+            for p, x in ((c.k1_pages, k1), (c.k2_pages, k2), (c.v_pages, v)):
+                assert torch.equal(p[pages, :, at % 16], x[i, :, :m].transpose(0, 1))
+            assert bool((c.positions[i, :, n:n + m] == at).all()) and not bool(c.weights[i, :, n:n + m].any())
+        assert c.lengths.tolist() == [n + m for n, m in zip([0, 30, 700, 9], gets)] == c.next_position.tolist()
+        assert sum(int(torch.isfinite(p[..., 0]).sum()) for p in (c.k1_pages, c.k2_pages, c.v_pages)) == 3 * h * sum(gets)
+
+
 EVICT = [
     # lengths, keep, recent, weights
     ([40, 33, 32, 0, 5], 32, 0, "random"),

@@ -14,7 +14,7 @@ LIB_PATH = os.environ.get("DIFFATTN_LIBRARY") or os.path.join(PKG_DIR, "libdiffa
 
 EXPORTS = ("diffattn_fwd", "diffattn_bwd", "diffattn_bwd_stages", "diffattn_bwd_static", "diffattn_lambda_fwd", "diffattn_lambda_bwd", "diffattn_workspace_bytes", "diffattn_status",
            "diffattn_last_error", "diffattn_version", "diffattn_supports",
-           "diffattn_cache_append", "diffattn_cache_attend", "diffattn_cache_evict", "diffattn_cache_workspace_bytes")
+           "diffattn_cache_append", "diffattn_cache_reset", "diffattn_cache_attend", "diffattn_cache_evict", "diffattn_cache_workspace_bytes")
 
 ERR_NAMES = {
     0: "OK", -1: "NULL_PTR", -2: "BAD_STRUCT", -3: "BAD_SHAPE", -4: "UNSUPPORTED_D", -5: "BAD_STRIDE",
@@ -70,7 +70,7 @@ class DiffAttnCacheParams(C.Structure):
         ("lambda_scale", C.c_void_p), ("lambda_dtype", C.c_int32), ("rms_norm", C.c_int32),
         ("sm_scale", C.c_float), ("lambda_init", C.c_float), ("eps", C.c_float), ("keep", C.c_int32),
         ("gain", C.c_void_p), ("y", C.c_void_p), ("recent", C.c_int32), ("reserved", C.c_int32),
-        ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64), ("counter", C.c_void_p),
     ]
 
 
@@ -95,11 +95,13 @@ def _load() -> C.CDLL:
         lib.diffattn_lambda_fwd.restype = C.c_int
         lib.diffattn_lambda_bwd.argtypes = [C.c_int32, C.c_void_p, C.c_int32] + [C.c_void_p] * 10
         lib.diffattn_lambda_bwd.restype = C.c_int
-    lib.has_cache = all(hasattr(lib, "diffattn_cache_" + name) for name in ("append", "attend", "evict", "workspace_bytes"))
+    lib.has_cache = all(hasattr(lib, "diffattn_cache_" + name) for name in ("append", "reset", "attend", "evict", "workspace_bytes"))
     if lib.has_cache:
         for fn in (lib.diffattn_cache_append, lib.diffattn_cache_attend, lib.diffattn_cache_evict):
             fn.argtypes = [C.POINTER(DiffAttnCacheParams)]
             fn.restype = C.c_int
+        lib.diffattn_cache_reset.argtypes = [C.c_int32, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p]
+        lib.diffattn_cache_reset.restype = C.c_int
         lib.diffattn_cache_workspace_bytes.argtypes = [C.POINTER(DiffAttnCacheParams), C.c_int32]
         lib.diffattn_cache_workspace_bytes.restype = C.c_uint64
     lib.diffattn_workspace_bytes.argtypes = [C.POINTER(DiffAttnParams)]

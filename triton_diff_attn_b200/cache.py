@@ -57,11 +57,11 @@ class DiffAttnCache:
     next_position       int32 [batch]: tokens the sequence has had.
     weights             float32 [batch, heads, slots] or None: the attention weight each token has gathered (`attend`).
 
-    All of these are the caller's to read and to write between calls (a new page, a sequence that starts anew: `lengths[b] = 0`,
+    All of these are the caller's to read and to write (in place) between calls (a new page, a sequence that starts anew: `lengths[b] = 0`,
     `next_position[b] = 0`).  They stay on the device and are not checked on the host: a length outside [0, slots], a page outside the pool or
     a token that finds its sequence full touches no memory it should not, leaves that call's results undefined and makes
     `device_status()` raise.  Slots that a call writes must belong to one sequence.  Calls on one cache that write it (all but
-    `attend` without a token and without weights) have to be ordered, as any writes to one tensor."""
+    `attend` without a token and without weights) have to be ordered, as any writes to one tensor; that goes for replays of captured calls too."""
 
     def __init__(self, batch: int, heads: int, head_dim: int, max_tokens: int, *, page_size: int = 64, track_weights: bool = False,
                  dtype=torch.float16, device=None):
@@ -136,6 +136,7 @@ class DiffAttnCache:
                 raise ValueError(f"{name} requires a gradient: the cache has no backward pass")
         self._k1_pages, self._k2_pages, self._v_pages, self._page_table = k1_pages, k2_pages, v_pages, page_table
         self._lengths, self._positions, self._next_position, self._weights = lengths, positions, next_position, weights
+        self._counter = lengths.new_zeros(1)      # every writing call leaves it 0
         self._shape = (batch, heads, d)
         self._device, self._index, self._dtype = device, k1_pages.get_device(), k1_pages.dtype
         p = _lib.DiffAttnCacheParams()
@@ -148,6 +149,15 @@ class DiffAttnCache:
         p.vp_stride_page, p.vp_stride_head, p.vp_stride_slot, _ = v_pages.stride()
         p.table_stride = page_table.stride(0)
         p.sm_scale, p.eps = 1.0 / math.sqrt(d), EPS
+        # the tensors stay where they are for the cache's life (and their memory with it, whatever becomes of the tensor objects)
+        p.k1_pages, p.k2_pages, p.v_pages, p.page_table, p.lengths, p.counter = (t.data_ptr() for t in (
+            k1_pages, k2_pages, v_pages, page_table, lengths, self._counter))
+        if positions is not None:
+            p.positions, p.next_position = positions.data_ptr(), next_position.data_ptr()
+        if weights is not None:
+            p.weights = weights.data_ptr()
+        self._memory = [t.untyped_storage() for t in (k1_pages, k2_pages, v_pages, page_table, lengths, positions, next_position, weights) if t is not None]
+        self._y = k1_pages.new_empty((batch, heads, 1, 2 * d))      # (a pattern: empty_like is the cheapest way to a new one)
         self._sizes = p
         self._attend_bytes = int(_lib.lib.diffattn_cache_workspace_bytes(self._params(), _lib.CACHE_ATTEND))
 
@@ -163,13 +173,7 @@ class DiffAttnCache:
 
     def _params(self):
         p = _lib.DiffAttnCacheParams.from_buffer_copy(self._sizes)      # a copy per call: calls of several threads do not share it
-        p.stream = torch._C._cuda_getCurrentRawStream(p.device)
-        p.k1_pages, p.k2_pages, p.v_pages = self._k1_pages.data_ptr(), self._k2_pages.data_ptr(), self._v_pages.data_ptr()
-        p.page_table, p.lengths = self._page_table.data_ptr(), self._lengths.data_ptr()
-        if self._positions is not None:
-            p.positions, p.next_position = self._positions.data_ptr(), self._next_position.data_ptr()
-        if self._weights is not None:
-            p.weights = self._weights.data_ptr()
+        p.stream = torch._C._cuda_getCurrentRawStream(self._index)
         return p
 
     def _check(self, name, t, rows, width):
@@ -207,7 +211,8 @@ class DiffAttnCache:
 
     def reset(self) -> None:
         """Every sequence starts anew: nothing is cached."""
-        torch._foreach_zero_([t for t in (self._lengths, self._next_position) if t is not None])      # one launch
+        _lib.check(_lib.lib.diffattn_cache_reset(self._index, torch._C._cuda_getCurrentRawStream(self._index), self._shape[0], self._sizes.lengths,
+                                                 self._sizes.next_position), "diffattn_cache_reset")
 
     def append(self, k1, k2, v, counts=None) -> None:
         """Stores the tokens k1, k2 [B, H, T, D], v [B, H, T, 2D] behind each sequence's last one.  `counts` (an integer tensor [B]): sequence b
@@ -238,7 +243,7 @@ class DiffAttnCache:
         A cache with `weights` adds |P1 - lambda P2| to each token's.
 
         A sequence that is not in use has length 0; a step stores a token there like everywhere (set its length back to 0 if that matters)."""
-        batch, heads, d = self._shape
+        d = self._shape[2]
         self._check("q1", q1, 1, d)
         self._check("q2", q2, 1, d)
         lam = lambda_scale
@@ -260,7 +265,7 @@ class DiffAttnCache:
             if gain.dtype is not torch.float32 or gain.stride(0) != 1:
                 gain = gain.detach().to(torch.float32).contiguous()
             p.gain = gain.data_ptr()
-        y = self._k1_pages.new_empty((batch, heads, 1, 2 * d))
+        y = torch.empty_like(self._y)
         p.y = y.data_ptr()
         ws = self._workspace(p, self._attend_bytes)  # noqa: F841
         _lib.check(_lib.lib.diffattn_cache_attend(p), "diffattn_cache_attend")
@@ -280,5 +285,6 @@ class DiffAttnCache:
         Pages behind the new lengths are free again."""
         p = self._params()
         p.keep, p.recent = int(keep), int(recent)
-        ws = self._workspace(p, int(_lib.lib.diffattn_cache_workspace_bytes(p, _lib.CACHE_EVICT)))  # noqa: F841
+        nbytes = int(_lib.lib.diffattn_cache_workspace_bytes(p, _lib.CACHE_EVICT))
+        ws = self._workspace(p, nbytes) if nbytes else None  # noqa: F841
         _lib.check(_lib.lib.diffattn_cache_evict(p), "diffattn_cache_evict")

@@ -33,6 +33,7 @@ struct CacheArgs {
   long long table_stride;
   int* lengths;                      // [b]
   int* next_position;                // [b] or null: tokens that the sequence has had, with those evicted
+  int* counter;                      // one, 0 between calls: see cache_last_block
   int* positions;                    // [b][h][slots] or null: the position of the token in each slot
   float* weights;                    // [b][h][slots] or null: accumulated attention weights
   uint4* k1; uint4* k2; uint4* v;    // the pools; strides in 16-byte pieces
@@ -69,15 +70,41 @@ __device__ __forceinline__ uint4* cache_piece(const CacheArgs& c, int page, int 
   return c.v + page * c.v_page + head * c.v_head + in_page * c.v_slot + (part - 2 * KP);
 }
 
+// The lengths change when every CTA has read them.  One warp of each takes a ticket once its CTA has (behind a barrier), and where it is the last
+// one this returns true, to the whole warp: it changes them.  The counter is 0 again then.  Writing calls on a cache are ordered, so one counter does.
+// A second kernel instead costs 2.7 us on the host and 1.5 on the GPU; where many CTAs come and go the ticket costs more than that (4096 of them, B4
+// H16 N2048 D64: 30 us instead of 26), so large appends have the second kernel.
+__device__ __forceinline__ bool cache_last_block(const CacheArgs& c) {
+  int ticket = 0;
+  if ((threadIdx.x & 31) == 0) {
+    __threadfence();
+    ticket = atomicAdd(c.counter, 1);
+  }
+  const bool last = __shfl_sync(0xffffffffu, ticket, 0) == int(gridDim.x * gridDim.y) - 1;
+  if (last) {
+    __threadfence();
+    if ((threadIdx.x & 31) == 0) *c.counter = 0;
+  }
+  return last;
+}
+
 struct CacheAppendArgs {
   CacheArgs c;
   int t;                             // rows given per (sequence, head)
+  int take_tickets;                  // the storing kernel moves the lengths on itself
   const int* counts;                 // [b] or null (all t): how many of them sequence b gets
   const uint4* k1; const uint4* k2; const uint4* v;
   long long k_b, k_h, k_t, v_b, v_h, v_t;      // in 16-byte pieces
 };
 
-__device__ __forceinline__ int append_count(const CacheAppendArgs& a, int b) { return a.counts ? min(max(a.counts[b], 0), a.t) : a.t; }
+__device__ __forceinline__ int append_count(const CacheAppendArgs& a, int b) {
+  return a.counts ? min(max(a.counts[b], 0), a.t) : a.t;
+}
+__device__ __forceinline__ void append_advance(const CacheAppendArgs& a, int b) {
+  const int len = cache_length(a.c, b), stored = min(append_count(a, b), a.c.slots - len);
+  a.c.lengths[b] = len + stored;
+  if (a.c.next_position) a.c.next_position[b] += stored;
+}
 
 // Where the rows of one block's round lie: found by one thread a row (two divisions' worth of arithmetic, a page, 64-bit products), read by
 // the D / 2 threads that move its pieces.  With every thread finding its own address the kernels here were bound by that: 213 instructions a warp for
@@ -123,7 +150,6 @@ __global__ void __launch_bounds__(APPEND_THREADS) diffattn_cache_append_kernel(c
   const int part = threadIdx.x % PARTS;
   const int first = blockIdx.x * BLOCK, row = threadIdx.x / PARTS;
   const int count = append_count(a, b);
-  if (first >= count) return;
   const uint4* src;
   long long step;
   if (part < D / 4) {
@@ -152,21 +178,28 @@ __global__ void __launch_bounds__(APPEND_THREADS) diffattn_cache_append_kernel(c
     }
   }
   __syncthreads();
+  if (a.take_tickets && threadIdx.x >= APPEND_THREADS - 32 && cache_last_block(c))
+    for (int s = threadIdx.x & 31; s < c.b; s += 32) append_advance(a, s);
   const Piece<D> piece(c, part);
 #pragma unroll
   for (int i = 0; i < APPEND_UNROLL; ++i)
     if (places.k[row + i * ROWS] >= 0) *piece.at(places, row + i * ROWS) = x[i];
 }
 
-// The lengths move on once every row is stored (the kernel above reads them).
 __global__ void __launch_bounds__(APPEND_THREADS) diffattn_cache_advance_kernel(const CacheAppendArgs a) {
   griddep_wait();
   griddep_launch();
   const int b = blockIdx.x * APPEND_THREADS + threadIdx.x;
-  if (b >= a.c.b) return;
-  const int len = cache_length(a.c, b), stored = min(append_count(a, b), a.c.slots - len);
-  a.c.lengths[b] = len + stored;
-  if (a.c.next_position) a.c.next_position[b] += stored;
+  if (b < a.c.b) append_advance(a, b);
+}
+
+__global__ void __launch_bounds__(APPEND_THREADS) diffattn_cache_reset_kernel(int* lengths, int* next_position, int n) {
+  griddep_wait();
+  griddep_launch();
+  const int b = blockIdx.x * APPEND_THREADS + threadIdx.x;
+  if (b >= n) return;
+  lengths[b] = 0;
+  if (next_position) next_position[b] = 0;
 }
 
 }  // namespace da

@@ -119,8 +119,14 @@ __global__ void __launch_bounds__(SELECT_THREADS) diffattn_cache_select_kernel(c
   const int bh = blockIdx.x, b = bh / c.h, tid = threadIdx.x, lane = tid & 31;
   const int newest_from = c.next_position[b] - a.recent;
   const int len = cache_length(c, b);
+  if (a.moves_at_once) {
+    __syncthreads();
+    if (tid >= SELECT_THREADS - 32 && cache_last_block(c))
+      for (int s = lane; s < c.b; s += 32)
+        if (c.lengths[s] > a.keep) c.lengths[s] = a.keep;
+  }
   if (len <= a.keep) {
-    if (tid == 0) a.count[bh] = 0;
+    if (tid == 0 && !a.moves_at_once) a.count[bh] = 0;
     return;
   }
   for (int i = tid; i < 4 * 256; i += SELECT_THREADS) hist[0][i] = 0;
@@ -227,16 +233,16 @@ __global__ void __launch_bounds__(SELECT_THREADS) diffattn_cache_select_kernel(c
   __syncthreads();
   if (a.moves_at_once) {
     move_rows<D, SELECT_THREADS>(a, places, bh, list, total, 0, 1);
-    total = 0;
-  } else if (list == near_list) {
-    for (int i = tid; i < total; i += SELECT_THREADS) a.moves[(long long)bh * a.most + i] = list[i];
+    return;
   }
+  if (list == near_list)
+    for (int i = tid; i < total; i += SELECT_THREADS) a.moves[(long long)bh * a.most + i] = list[i];
   if (tid == 0) a.count[bh] = total;
 }
 
 constexpr int MOVE_THREADS = 256;
 
-// Grid (wide, b * h): the moves that the selection wrote down.
+// Grid (wide, b * h): the moves that the selection wrote down, and the lengths.
 template <int D>
 __global__ void __launch_bounds__(MOVE_THREADS) diffattn_cache_move_kernel(const EvictArgs a) {
   __shared__ MovePlaces<D, MOVE_THREADS> places;
@@ -245,14 +251,6 @@ __global__ void __launch_bounds__(MOVE_THREADS) diffattn_cache_move_kernel(const
   const int bh = blockIdx.y, b = bh / a.c.h;
   move_rows<D, MOVE_THREADS>(a, places, bh, a.moves + (long long)bh * a.most, a.count[bh], blockIdx.x, gridDim.x);
   if (blockIdx.x == 0 && bh == b * a.c.h && threadIdx.x == 0 && a.c.lengths[b] > a.keep) a.c.lengths[b] = a.keep;
-}
-
-// The lengths alone, where the selection has moved everything.
-__global__ void __launch_bounds__(MOVE_THREADS) diffattn_cache_shorten_kernel(const EvictArgs a) {
-  griddep_wait();
-  griddep_launch();
-  const int b = blockIdx.x * MOVE_THREADS + threadIdx.x;
-  if (b < a.c.b && a.c.lengths[b] > a.keep) a.c.lengths[b] = a.keep;
 }
 
 }  // namespace da

@@ -50,6 +50,20 @@ AttendSpace attend_space(const DiffAttnCacheParams* p) {
 }
 int evict_most(const DiffAttnCacheParams* p) { return std::min(p->keep, p->max_pages * p->page_size - p->keep); }
 
+// the selecting kernel moves rows itself: a few a CTA, or CTAs for every SM
+bool evict_at_once(const DiffAttnCacheParams* p) { return evict_most(p) <= 64 || p->B * p->H >= sm_count(p->device); }
+struct EvictSpace {
+  uint64_t moves, bytes;
+};
+EvictSpace evict_space(const DiffAttnCacheParams* p) {
+  const uint64_t bh = uint64_t(p->B) * p->H, most = uint64_t(evict_most(p));
+  const bool at_once = evict_at_once(p);
+  EvictSpace s;
+  s.moves = at_once ? 0 : round256(4 * bh);
+  s.bytes = s.moves + (at_once && most <= da::SELECT_LIST ? 0 : round256(8 * bh * most));
+  return s;
+}
+
 bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 bool good_stride(int64_t s, bool used) { return !used || (s > 0 && s % 8 == 0); }
 
@@ -83,9 +97,9 @@ int check_cache(const DiffAttnCacheParams* p) {
     if (!ptrs[i]) return fail(DIFFATTN_ERR_NULL_PTR, "%s is NULL", names[i]);
   for (int i = 0; i < 3; ++i)
     if (!aligned16(ptrs[i])) return fail(DIFFATTN_ERR_MISALIGNED, "%s is not 16-byte aligned", names[i]);
-  const void* words[] = {p->page_table, p->lengths, p->next_position, p->positions, p->weights};
+  const void* words[] = {p->page_table, p->lengths, p->next_position, p->positions, p->weights, p->counter};
   for (const void* w : words)
-    if (!aligned_to(w, 4)) return fail(DIFFATTN_ERR_MISALIGNED, "page_table, lengths, next_position, positions and weights must be 4-byte aligned");
+    if (!aligned_to(w, 4)) return fail(DIFFATTN_ERR_MISALIGNED, "page_table, lengths, next_position, positions, weights and counter must be 4-byte aligned");
   if ((p->positions != nullptr) != (p->next_position != nullptr)) return fail(DIFFATTN_ERR_NULL_PTR, "positions and next_position go together");
   const int64_t st[] = {p->kp_stride_page, p->kp_stride_head, p->kp_stride_slot, p->vp_stride_page, p->vp_stride_head, p->vp_stride_slot};
   const bool used[] = {p->num_pages > 1, p->H > 1, p->page_size > 1, p->num_pages > 1, p->H > 1, p->page_size > 1};
@@ -114,6 +128,7 @@ int check_tokens(const DiffAttnCacheParams* p, bool rows) {
 }
 
 int check_cache_workspace(const DiffAttnCacheParams* p, uint64_t need) {
+  if (need == 0) return DIFFATTN_OK;
   if (!p->workspace || p->workspace_bytes < need)
     return fail(DIFFATTN_ERR_WORKSPACE, "workspace %llu bytes, need %llu", (unsigned long long)p->workspace_bytes, (unsigned long long)need);
   if (reinterpret_cast<uintptr_t>(p->workspace) & 255) return fail(DIFFATTN_ERR_MISALIGNED, "workspace not 256-byte aligned");
@@ -121,9 +136,9 @@ int check_cache_workspace(const DiffAttnCacheParams* p, uint64_t need) {
 }
 
 int cache_on_device(const DiffAttnCacheParams* p) {
-  const void* ptrs[] = {p->k1_pages, p->k2_pages, p->v_pages, p->page_table, p->lengths, p->next_position, p->positions, p->weights};
-  const char* names[] = {"k1_pages", "k2_pages", "v_pages", "page_table", "lengths", "next_position", "positions", "weights"};
-  for (int i = 0; i < 8; ++i)
+  const void* ptrs[] = {p->k1_pages, p->k2_pages, p->v_pages, p->page_table, p->lengths, p->next_position, p->positions, p->weights, p->counter};
+  const char* names[] = {"k1_pages", "k2_pages", "v_pages", "page_table", "lengths", "next_position", "positions", "weights", "counter"};
+  for (int i = 0; i < 9; ++i)
     if (int rc = check_on_device(ptrs[i], p->device, names[i])) return rc;
   return DIFFATTN_OK;
 }
@@ -137,7 +152,7 @@ da::CacheArgs cache_args(const DiffAttnCacheParams* p) {
   c.slots = p->max_pages * p->page_size;
   c.page_magic = p->page_size > 1 ? uint32_t(((1ull << 32) + p->page_size - 1) / p->page_size) : 0u;
   c.page_table = p->page_table; c.table_stride = p->table_stride;
-  c.lengths = p->lengths; c.next_position = p->next_position; c.positions = p->positions; c.weights = p->weights;
+  c.lengths = p->lengths; c.counter = p->counter; c.next_position = p->next_position; c.positions = p->positions; c.weights = p->weights;
   c.k1 = static_cast<uint4*>(p->k1_pages); c.k2 = static_cast<uint4*>(p->k2_pages); c.v = static_cast<uint4*>(p->v_pages);
   c.k_page = pieces(p->kp_stride_page, p->num_pages > 1); c.k_head = pieces(p->kp_stride_head, p->H > 1); c.k_slot = pieces(p->kp_stride_slot, p->page_size > 1);
   c.v_page = pieces(p->vp_stride_page, p->num_pages > 1); c.v_head = pieces(p->vp_stride_head, p->H > 1); c.v_slot = pieces(p->vp_stride_slot, p->page_size > 1);
@@ -187,8 +202,7 @@ int evict_launch(const DiffAttnCacheParams* p, const da::EvictArgs& a) {
   const int bh = p->B * p->H;
   if ((rc = set_smem(da::diffattn_cache_select_kernel<D>, da::SELECT_MOST_KEYS * 4, p->device))) return rc;
   if ((rc = launch(da::diffattn_cache_select_kernel<D>, dim3(bh), da::SELECT_THREADS, a.cached_keys ? a.c.slots * 4 : 0, stream, true, a))) return rc;
-  if (a.moves_at_once)
-    return launch(da::diffattn_cache_shorten_kernel, dim3((p->B + da::MOVE_THREADS - 1) / da::MOVE_THREADS), da::MOVE_THREADS, 0, stream, true, a);
+  if (a.moves_at_once) return DIFFATTN_OK;
   // as many CTAs as the SMs hold, spread over the (sequence, head)s, but no more than there can be moves for
   const int rows = da::MovePlaces<D, da::MOVE_THREADS>::BLOCK;
   const int wide = std::max(1, std::min((a.most + rows - 1) / rows, (sm_count(p->device) * 8 + bh - 1) / bh));
@@ -204,8 +218,7 @@ uint64_t diffattn_cache_workspace_bytes(const DiffAttnCacheParams* p, int32_t op
   if (operation == DIFFATTN_CACHE_ATTEND) return attend_space(p).bytes;
   if (operation == DIFFATTN_CACHE_EVICT) {
     if (p->keep < 1 || p->keep > p->max_pages * p->page_size) return 0;
-    const uint64_t bh = uint64_t(p->B) * p->H;
-    return round256(4 * bh) + round256(8 * bh * evict_most(p));
+    return evict_space(p).bytes;
   }
   return 0;
 }
@@ -216,6 +229,7 @@ int diffattn_cache_append(const DiffAttnCacheParams* p) {
   if (p->T < 0 || p->T > INT32_MAX - 1024) return fail(DIFFATTN_ERR_BAD_SHAPE, "T=%d", p->T);
   if (p->T == 0) return DIFFATTN_OK;
   if ((rc = check_tokens(p, true))) return rc;
+  if (!p->counter) return fail(DIFFATTN_ERR_NULL_PTR, "counter is NULL");
   if (!aligned_to(p->counts, 4)) return fail(DIFFATTN_ERR_MISALIGNED, "counts is not 4-byte aligned");
   DeviceGuard guard;
   if ((rc = guard.enter(p->device))) return rc;
@@ -234,8 +248,22 @@ int diffattn_cache_append(const DiffAttnCacheParams* p) {
   const int rows = da::APPEND_THREADS / (p->D / 2) * da::APPEND_UNROLL;
   const dim3 grid((p->T + rows - 1) / rows, p->B * p->H);
   auto kernel = p->D == 32 ? da::diffattn_cache_append_kernel<32> : p->D == 64 ? da::diffattn_cache_append_kernel<64> : da::diffattn_cache_append_kernel<128>;
-  if ((rc = launch(kernel, grid, da::APPEND_THREADS, 0, stream, true, a))) return rc;
+  a.take_tickets = (long long)grid.x * grid.y <= 4 * sm_count(p->device) ? 1 : 0;
+  if ((rc = launch(kernel, grid, da::APPEND_THREADS, 0, stream, true, a)) || a.take_tickets) return rc;
   return launch(da::diffattn_cache_advance_kernel, dim3((p->B + da::APPEND_THREADS - 1) / da::APPEND_THREADS), da::APPEND_THREADS, 0, stream, true, a);
+}
+
+int diffattn_cache_reset(int32_t device, void* stream, int32_t B, int32_t* lengths, int32_t* next_position) {
+  if (B < 0) return fail(DIFFATTN_ERR_BAD_SHAPE, "B=%d", B);
+  if (B == 0) return DIFFATTN_OK;
+  if (!lengths) return fail(DIFFATTN_ERR_NULL_PTR, "lengths is NULL");
+  if (!aligned_to(lengths, 4) || !aligned_to(next_position, 4)) return fail(DIFFATTN_ERR_MISALIGNED, "lengths and next_position must be 4-byte aligned");
+  DeviceGuard guard;
+  int rc = guard.enter(device);
+  if (rc) return rc;
+  if ((rc = check_on_device(lengths, device, "lengths")) || (rc = check_on_device(next_position, device, "next_position"))) return rc;
+  return launch(da::diffattn_cache_reset_kernel, dim3((B + da::APPEND_THREADS - 1) / da::APPEND_THREADS), da::APPEND_THREADS, 0,
+                static_cast<cudaStream_t>(stream), true, lengths, next_position, B);
 }
 
 int diffattn_cache_attend(const DiffAttnCacheParams* p) {
@@ -294,21 +322,20 @@ int diffattn_cache_evict(const DiffAttnCacheParams* p) {
   if (p->keep < 1 || p->keep > p->max_pages * p->page_size || p->recent < 0 || p->recent > p->keep)
     return fail(DIFFATTN_ERR_BAD_SHAPE, "keep=%d must lie in [1, %d], recent=%d in [0, keep]", p->keep, p->max_pages * p->page_size, p->recent);
   if (rc == 1) return DIFFATTN_OK;
-  if (!p->positions) return fail(DIFFATTN_ERR_NULL_PTR, "evict needs positions and next_position");
+  if (!p->positions || !p->counter) return fail(DIFFATTN_ERR_NULL_PTR, "evict needs positions, next_position and counter");
   DeviceGuard guard;
   if ((rc = guard.enter(p->device))) return rc;
-  if ((rc = check_cache_workspace(p, diffattn_cache_workspace_bytes(p, DIFFATTN_CACHE_EVICT)))) return rc;
+  const EvictSpace space = evict_space(p);
+  if ((rc = check_cache_workspace(p, space.bytes))) return rc;
   if ((rc = cache_on_device(p))) return rc;
-  if ((rc = check_on_device(p->workspace, p->device, "workspace"))) return rc;
-  const int bh = p->B * p->H;
+  if (space.bytes && (rc = check_on_device(p->workspace, p->device, "workspace"))) return rc;
   da::EvictArgs a;
   a.c = cache_args(p);
   a.keep = p->keep; a.recent = p->recent; a.most = evict_most(p);
   a.count = static_cast<int*>(p->workspace);
-  a.moves = reinterpret_cast<int2*>(static_cast<uint8_t*>(p->workspace) + round256(4 * uint64_t(bh)));
+  a.moves = reinterpret_cast<int2*>(static_cast<uint8_t*>(p->workspace) + space.moves);
   a.cached_keys = a.c.slots <= da::SELECT_MOST_KEYS ? 1 : 0;
-  const int sms = sm_count(p->device);
-  a.moves_at_once = a.most <= 64 || bh >= sms ? 1 : 0;
+  a.moves_at_once = evict_at_once(p) ? 1 : 0;
   return p->D == 32 ? evict_launch<32>(p, a) : p->D == 64 ? evict_launch<64>(p, a) : evict_launch<128>(p, a);
 }
 
