@@ -595,6 +595,16 @@ def test_refusals(pkg):
                       (0, c.k1_pages.float(), ValueError), (3, c.page_table.long(), ValueError), (4, c.lengths.long(), ValueError), (3, c.page_table.cpu(), RuntimeError)):
         with pytest.raises(err):
             take(*(t if i == k else x for k, x in enumerate(good)))
+    flat = torch.zeros(64 * 200, dtype=torch.float16, device=DEV)
+    lapped = flat.as_strided((2, 2, 16, 64), (2048, 32, 64, 1))       # heads half a row apart
+    with pytest.raises(ValueError):
+        take(lapped, lapped, torch.zeros(2, 2, 16, 128, dtype=torch.float16, device=DEV), c.page_table, c.lengths)
+    with pytest.raises(ValueError):
+        take(c.k1_pages[:0], c.k2_pages[:0], c.v_pages[:0], c.page_table, c.lengths)
+    with pytest.raises(ValueError):
+        pkg.DiffAttnCache(5000, 1, 32, 16, device=DEV)
+    column = take(*good[:3], c.page_table[:, :1], c.lengths)           # (a column of a wider table: rows of one entry)
+    assert column.slots == 16
     with pytest.raises(ValueError):
         take(*good, positions=c.positions)
     with pytest.raises(ValueError):

@@ -110,7 +110,7 @@ class DiffAttnCache:
             raise ValueError("k2_pages must have the shape and strides of k1_pages")
         if tuple(v_pages.shape) != (pages, heads, page_size, 2 * d):
             raise ValueError(f"v_pages shape {tuple(v_pages.shape)} != {(pages, heads, page_size, 2 * d)}")
-        if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.shape[1] < 1 or page_table.stride(1) != 1:
+        if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.shape[1] < 1 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
             raise ValueError("page_table must be int32 [batch, max_pages] with contiguous rows")
         batch, max_pages = page_table.shape
         if batch > 1 and page_table.stride(0) < max_pages:
@@ -137,6 +137,8 @@ class DiffAttnCache:
         self._k1_pages, self._k2_pages, self._v_pages, self._page_table = k1_pages, k2_pages, v_pages, page_table
         self._lengths, self._positions, self._next_position, self._weights = lengths, positions, next_position, weights
         self._counter = lengths.new_zeros(1)      # every writing call leaves it 0
+        if not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream(device).synchronize()      # (the first call may come on another stream)
         self._shape = (batch, heads, d)
         self._device, self._index, self._dtype = device, k1_pages.get_device(), k1_pages.dtype
         p = _lib.DiffAttnCacheParams()
@@ -159,6 +161,7 @@ class DiffAttnCache:
         self._memory = [t.untyped_storage() for t in (k1_pages, k2_pages, v_pages, page_table, lengths, positions, next_position, weights) if t is not None]
         self._y = k1_pages.new_empty((batch, heads, 1, 2 * d))      # (a pattern: empty_like is the cheapest way to a new one)
         self._sizes = p
+        _lib.check(_lib.lib.diffattn_cache_append(p), "diffattn_cache_append")      # (T = 0: the checks of sizes and strides alone)
         self._attend_bytes = int(_lib.lib.diffattn_cache_workspace_bytes(self._params(), _lib.CACHE_ATTEND))
 
     k1_pages = property(lambda self: self._k1_pages)
