@@ -49,9 +49,10 @@ constexpr int MAX_B = 4096;                    // the prefix sums and lengths of
 template <int D>
 struct Geo {
   static constexpr int T = D == 32 ? 32 : 16;  // tokens per tile: 8 KB of K1, K2, V (D = 128: 16 KB)
-  static constexpr int WARPS = D == 128 ? 4 : 8, THREADS = WARPS * 32;
-  // Tiles in flight per warp: 128 KB of requests an SM.  Three are slower (B64 H16 ragged to 4096 D64: 206 us, two 190): the SMs get their share of
-  // HBM less evenly, and the last one counts.  One, with 12 warps: 183 there, but 33 instead of 31 at B1 H16 N16384.  Six warps: 207.
+  static constexpr int WARPS = D == 32 ? 8 : D == 64 ? 7 : 4, THREADS = WARPS * 32;
+  // Tiles in flight per warp.  Warps x slots is what an SM has asked for, 112 to 128 KB.  More is slower, because the SMs then get their share of HBM
+  // less evenly and the last one counts; fewer warps than this do not keep up.  B64 H16 ragged to 4096 D64: 7 x 2 180 us, 8 x 2 188, 8 x 3
+  // 206, 12 x 2 198, 12 x 1 183 (but B1 H16 N16384 33 instead of 30), 6 x 2 207.  D = 32: 7 x 2 32 us, 8 x 2 30; D = 128: 4 x 2 88, 6 x 2 95.
   static constexpr int SLOTS = 2;
   // a tile in shared memory: boxes of T rows of 128 bytes (K at D = 32: 64 bytes), swizzled by the engine: K1, K2, V
   static constexpr int K_ROW = D == 32 ? 64 : 128, K_BOXES = D == 128 ? 2 : 1, V_BOXES = D / 32;
