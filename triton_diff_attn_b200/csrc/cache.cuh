@@ -9,8 +9,7 @@
 
 namespace da {
 
-// what g_status[0] holds for a cache whose contents make no sense (sites of waits that gave up are below)
-constexpr int kCacheSite = 900;
+// what g_status[0] holds for a cache whose contents make no sense (sites of waits that gave up are below 900)
 constexpr int kCacheBadLength = 901, kCacheBadPage = 902, kCacheFull = 903;
 
 __device__ __noinline__ void cache_fault(int site, int b, int at) {

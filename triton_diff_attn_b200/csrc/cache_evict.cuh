@@ -6,8 +6,7 @@
 // the others, and a call that evicts a few tokens moves a few rows.
 //
 // The selection takes a CTA per (sequence, head): 8 bytes per token read, the rest in shared memory.  Where its moves are few, or the CTAs enough
-// to fill the GPU, it carries them out too; else it writes them down for a second kernel that spreads them over all SMs.  Either way the
-// lengths change in a kernel behind it, when every head has read them.
+// to fill the GPU, it carries them out too; else it writes them down for a second kernel that spreads them over all SMs.
 #pragma once
 #include "cache.cuh"
 
