@@ -184,9 +184,9 @@ int attend_launch(const DiffAttnCacheParams* p, da::AttendArgs& a) {
   auto weights = [&](int blocks) { return TRACK ? bh * ((blocks + bh - 1) / bh) : 0; };
   a.join_blocks = bh;
   if (pieces > 40) return launch(da::diffattn_cache_join_kernel<D, 1024, BF, TRACK>, dim3(bh + weights(sms)), 1024, 0, stream, true, a);
-  if (pieces > 2) return launch(da::diffattn_cache_join_kernel<D, 256, BF, TRACK>, dim3(bh + weights(4 * sms)), 256, 0, stream, true, a);
+  if (pieces > 2) return launch(da::diffattn_cache_join_kernel<D, 256, BF, TRACK>, dim3(bh + weights(2 * sms)), 256, 0, stream, true, a);
   a.join_blocks = (bh + da::JOIN_FEW / 32 - 1) / (da::JOIN_FEW / 32);
-  return launch(da::diffattn_cache_join_few_kernel<D, BF, TRACK>, dim3(a.join_blocks + weights(4 * sms)), da::JOIN_FEW, 0, stream, true, a);
+  return launch(da::diffattn_cache_join_few_kernel<D, BF, TRACK>, dim3(a.join_blocks + weights(2 * sms)), da::JOIN_FEW, 0, stream, true, a);
 }
 template <int D>
 int attend_launch(const DiffAttnCacheParams* p, da::AttendArgs& a) {
