@@ -190,7 +190,8 @@ typedef struct DiffAttnCacheParams {
   const void* k1; const void* k2; const void* v;
   int64_t k_stride_b, k_stride_h, k_stride_t;
   int64_t v_stride_b, v_stride_h, v_stride_t;
-  const int32_t* counts;           /* append: [B] rows that each sequence gets (0 .. T), or NULL: T */
+  const int32_t* counts;           /* [B] or NULL.  append: rows that each sequence gets, 0 .. T (NULL: T); attend with a token: sequences
+                                      with 0 get none, the others theirs */
   /* attend */
   const void* q1; const void* q2;  /* [B, H, D], one set of strides */
   int64_t q_stride_b, q_stride_h;
@@ -215,7 +216,7 @@ int diffattn_cache_append(const DiffAttnCacheParams* p);
 int diffattn_cache_reset(int32_t device, void* stream, int32_t B, int32_t* lengths, int32_t* next_position);
 /* y = (softmax(s q1 K1^T) - lambda softmax(s q2 K2^T)) V, norm and gain as diffattn_fwd, for one query per (sequence, head) over the
  * sequence's tokens; y = 0 where it has none.  With k1, k2, v (one token per sequence) that token is stored first, as append
- * does, and takes part.  weights, where given, grow by |P_1 - lambda P_2|.  Bit-reproducible on a given GPU model. */
+ * does, and takes part; a sequence that gets none by `counts` is as in a call without a token (nothing of it is written but weights).  weights, where given, grow by |P_1 - lambda P_2|.  Bit-reproducible on a given GPU model. */
 int diffattn_cache_attend(const DiffAttnCacheParams* p);
 /* Cuts every sequence longer than `keep` back to `keep` tokens, per head: those of the last `recent` positions stay, then those
  * with the largest weights (ties: the lowest slot; NaN counts as the largest), without weights those of the largest positions.  Survivors in slots

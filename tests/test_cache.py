@@ -41,7 +41,7 @@ BAD = [
     (ALL, "page_table", 0, -1), (ALL, "lengths", 0, -1), (ALL, "v_pages", 0x10008, -6), (ALL, "kp_stride_head", 60, -5), (ALL, "kp_stride_page", 0, -5),
     (ALL, "vp_stride_slot", 64, -5), (ALL, "table_stride", 3, -5), (ALL, "positions", 0, -1), (ALL, "device", 64, -3), (ALL, "device", -1, -3),
     (("append",), "T", -1, -3), (("append", "attend"), "k2", 0, -1), (("append", "attend"), "v", 0x10008, -6), (("append", "attend"), "v_stride_h", 12, -5),
-    (("append", "evict"), "counter", 0, -1), (ALL, "counter", 0x10002, -6), (("append",), "T", 2 ** 31 - 1, -3), (("append",), "counts", 0x10002, -6), (ALL, "lengths", 0x10002, -6), (ALL, "page_table", 0x10001, -6),
+    (("append", "evict"), "counter", 0, -1), (ALL, "counter", 0x10002, -6), (("append",), "T", 2 ** 31 - 1, -3), (("append", "attend"), "counts", 0x10002, -6), (ALL, "lengths", 0x10002, -6), (ALL, "page_table", 0x10001, -6),
     (ALL, "weights", 0x10002, -6), (("attend",), "y", 0x10002, -6), (("attend",), "gain", 0x10002, -6), (("attend",), "lambda_scale", 0x10002, -6),
     (("append",), "k_stride_t", 0, -5), (("attend",), "q1", 0, -1), (("attend",), "q2", 0x10004, -6), (("attend",), "q_stride_h", 4, -5),
     (("attend",), "lambda_dtype", 9, -7), (("attend",), "y", 0, -1), (("attend",), "lambda_scale", 0, -1),
@@ -119,23 +119,24 @@ def tile_shape(d, page):
     return t, r, 0
 
 
-def tiles_of(n, page, shape, token):
+def tiles_of(n, page, shape):
     t, _, per_page = shape
     if not per_page:
-        return -(-n // t) + token
+        return -(-n // t)
     full = n // page
-    return full * per_page + -(-(n - full * page) // t) + token
+    return full * per_page + -(-(n - full * page) // t)
 
 
-def tile_at(i, n_tiles, n, page, shape, token):
+def tile_at(i, n, page, shape):
     t, _, per_page = shape
-    if token and i == n_tiles - 1:
-        return n, 1, True
     slot, end = i * t, n
     if per_page:
         p = i // per_page
         slot, end = p * page + (i - p * per_page) * t, min(n, (p + 1) * page)
-    return slot, min(t, end - slot), False
+        new = i >= tiles_of(n, page, shape)
+    else:
+        new = slot >= n
+    return (n, 1, True) if new else (slot, min(t, end - slot), False)
 
 
 @pytest.mark.parametrize("d", [32, 64, 128])
@@ -146,10 +147,11 @@ def test_tiles_cover_every_token_once(d):
         assert t % box == 0 and box * (64 if d == 32 else 128) % 128 == 0 and (per_page or page % box == 0)
         for n in list(range(0, 3 * t + 2)) + [page - 1, page, page + 1, 4 * page, 4 * page + 1]:
             for token in (0, 1):
-                m, seen = tiles_of(n, page, shape, token), []
+                m, seen = tiles_of(n, page, shape) + token, []
                 for i in range(m):
-                    slot, valid, new = tile_at(i, m, n, page, shape, token)
+                    slot, valid, new = tile_at(i, n, page, shape)
                     assert 1 <= valid <= t
+                    assert new == (token == 1 and i == m - 1)
                     if new:
                         assert slot == n
                         continue
@@ -165,7 +167,7 @@ def test_tiles_cover_every_token_once(d):
         # the bound that the workspace is sized by
         slots = 4 * page
         most = (4 * per_page if per_page else -(-slots // t)) + 1
-        assert max(tiles_of(n, page, shape, 1) for n in range(slots + 1)) <= most
+        assert max(tiles_of(n, page, shape) + 1 for n in range(slots + 1)) <= most
 
 
 def test_pieces_of_the_line():

@@ -201,6 +201,43 @@ def test_attend_strided_queries_and_shared_pages(pkg):
     pkg.device_status(0)
 
 
+@pytest.mark.parametrize("d,page", [(64, 16), (32, 7), (128, 100)])
+@pytest.mark.parametrize("track", [False, True])
+def test_attend_some_get_a_token(pkg, d, page, track):
+    """A batch with rows that are not in use: no pages, no length, nothing of them written; others only look."""
+    lengths, counts = [0, 20, 0, 33, 48, 0, 7], [1, 1, 0, 0, 1, 0, 0]
+    c = make(pkg, lengths, 2, d, page, track=track, seed=page, room=1)
+    for i in (2, 5):
+        c.page_table[i] = -1
+    q1, q2, k1, k2, v = queries(7, 2, d, torch.float16, seed=d)
+    lam = torch.tensor([0.5], device=DEV)
+    before, old = snapshot(c), {"weights": None if c.weights is None else c.weights.clone()}
+    y = c.attend(q1, q2, lam, k1=k1, k2=k2, v=v, counts=torch.tensor(counts, device=DEV))
+    pkg.device_status(0)
+    for got in (0, 1):
+        at = [i for i in range(7) if counts[i] == got]
+        sub = type("C", (), dict(k1_pages=c.k1_pages, k2_pages=c.k2_pages, v_pages=c.v_pages, page_table=c.page_table[at],
+                                 weights=None if c.weights is None else c.weights[at]))
+        check_attend(sub, {"weights": None if c.weights is None else old["weights"][at]}, y[at], q1[at], q2[at], 0.5, [lengths[i] for i in at],
+                     tuple(x[at] for x in (k1, k2, v)) if got else None, rms=False)
+    assert c.lengths.tolist() == [n + m for n, m in zip(lengths, counts)] == c.next_position.tolist()
+    for i, (n, m) in enumerate(zip(lengths, counts)):
+        if m:
+            for t, x in zip((c.k1_pages, c.k2_pages, c.v_pages), (k1, k2, v)):
+                p = int(c.page_table[i, n // page])
+                assert torch.equal(t[p, :, n % page], x[i, :, 0])
+                t[p, :, n % page] = math.nan
+            assert bool((c.positions[i, :, n] == n).all())
+            c.positions[i, :, n] = -9
+        if track:
+            c.weights[i, :, :n + m] = old["weights"][i, :, :n + m]
+    c.lengths.copy_(torch.tensor(lengths, dtype=torch.int32)); c.next_position.copy_(c.lengths)
+    for a, w in zip(snapshot(c), before):
+        assert a is None or torch.equal(a, w)
+    with pytest.raises(ValueError):
+        c.attend(q1, q2, lam, counts=torch.tensor(counts, device=DEV))
+
+
 def test_attend_far_pages(pkg):
     """Rows more than 2^32 bytes behind the pool's base."""
     page, d, h = 256, 128, 1

@@ -207,6 +207,18 @@ class DiffAttnCache:
         p.v_stride_b, p.v_stride_h, p.v_stride_t, _ = sv
         return k1, k2, v
 
+    def _counts(self, p, counts):
+        if not isinstance(counts, torch.Tensor):
+            raise TypeError("counts must be a tensor")
+        if counts.get_device() != self._index:
+            raise RuntimeError(f"counts is on {counts.device}, the cache on {self._device}")
+        if counts.dtype not in (torch.int32, torch.int64) or tuple(counts.shape) != (self._shape[0],):
+            raise ValueError(f"counts must be int32 or int64 of shape {(self._shape[0],)}")
+        if counts.dtype is not torch.int32 or not counts.is_contiguous():
+            counts = counts.to(torch.int32).contiguous()
+        p.counts = counts.data_ptr()
+        return counts
+
     def _workspace(self, p, nbytes):
         ws = self._lengths.new_empty(max(nbytes, 256) // 4)
         p.workspace, p.workspace_bytes = ws.data_ptr(), nbytes
@@ -226,26 +238,20 @@ class DiffAttnCache:
         p.T = k1.shape[2]
         keep = self._tokens(p, k1, k2, v, p.T)  # noqa: F841  (copies stay until the call is enqueued)
         if counts is not None:
-            if not isinstance(counts, torch.Tensor):
-                raise TypeError("counts must be a tensor")
-            if counts.get_device() != self._index:
-                raise RuntimeError(f"counts is on {counts.device}, the cache on {self._device}")
-            if counts.dtype not in (torch.int32, torch.int64) or tuple(counts.shape) != (self._shape[0],):
-                raise ValueError(f"counts must be int32 or int64 of shape {(self._shape[0],)}")
-            if counts.dtype is not torch.int32 or not counts.is_contiguous():
-                counts = counts.to(torch.int32).contiguous()
-            p.counts = counts.data_ptr()
+            counts = self._counts(p, counts)
         _lib.check(_lib.lib.diffattn_cache_append(p), "diffattn_cache_append")
 
-    def attend(self, q1, q2, lambda_scale, lambda_init: float = 0.8, rms_norm: bool = False, gain=None, k1=None, k2=None, v=None):
+    def attend(self, q1, q2, lambda_scale, lambda_init: float = 0.8, rms_norm: bool = False, gain=None, k1=None, k2=None, v=None,
+               counts=None):
         """Differential attention of one query per sequence and head, q1, q2 [B, H, 1, D], over the sequence's tokens; returns [B, H, 1, 2D].
         lambda_scale, lambda_init, rms_norm and gain as in `MultiheadDiffAttnKernel`, scale 1/sqrt(D).  A sequence without tokens gives 0.
 
         With k1, k2 [B, H, 1, D] and v [B, H, 1, 2D] (all or none) that token is stored first, in the same launches, and takes part: the
         step of a generation.  Without them nothing is stored: a query over an encoder's states, say, that `append` put there.
-        A cache with `weights` adds |P1 - lambda P2| to each token's.
+        `counts` (an integer tensor [B]): only sequences with a positive one get their token; the others' state stays as it is, so the unused rows
+        of a batch (length 0, no pages) take part in nothing.
 
-        A sequence that is not in use has length 0; a step stores a token there like everywhere (set its length back to 0 if that matters)."""
+        A cache with `weights` adds |P1 - lambda P2| to each token's."""
         d = self._shape[2]
         self._check("q1", q1, 1, d)
         self._check("q2", q2, 1, d)
@@ -260,6 +266,10 @@ class DiffAttnCache:
         p = self._params()
         if k1 is not None or k2 is not None or v is not None:
             keep = self._tokens(p, k1, k2, v, 1)  # noqa: F841  (copies stay until the call is enqueued)
+            if counts is not None:
+                counts = self._counts(p, counts)
+        elif counts is not None:
+            raise ValueError("counts goes with a token: k1, k2 and v are missing")
         q1, q2, sq = _pair(q1, q2)
         p.q1, p.q2, p.q_stride_b, p.q_stride_h = q1.data_ptr(), q2.data_ptr(), sq[0], sq[1]
         p.lambda_scale, p.lambda_dtype = lam.data_ptr(), _LAMBDA_DTYPES[lam.dtype]

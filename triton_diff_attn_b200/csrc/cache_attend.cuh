@@ -24,6 +24,7 @@ struct AttendArgs {
   long long q_b, q_h;
   const uint4* nk1; const uint4* nk2; const uint4* nv;     // the new token (or null: the cache as it is)
   long long nk_b, nk_h, nv_b, nv_h;
+  const int* counts;                           // [b] or null: only sequences with a positive one get their token
   float scale_log2;                            // log2(e) / sqrt(D): scores are kept in base 2
   const void* lambda_ptr;
   int lambda_dtype, rms_norm;
@@ -100,31 +101,31 @@ __device__ __forceinline__ int divide(int n, int d, uint32_t magic) {      // as
   if ((long long)q * d > n) --q;
   return q;
 }
+// tiles of `len` cached tokens; a sequence that gets a token has one tile more, the last, for that alone
 template <int T>
 __device__ __forceinline__ int attend_tiles(const AttendArgs& a, int len) {
-  int n = (len + T - 1) / T;
-  if (a.tiles_per_page) {
-    const int full = cache_page(a.c, len);
-    n = full * a.tiles_per_page + (len - full * a.c.page_size + T - 1) / T;
-  }
-  return n + (a.nk1 != nullptr ? 1 : 0);
+  if (!a.tiles_per_page) return (len + T - 1) / T;
+  const int full = cache_page(a.c, len);
+  return full * a.tiles_per_page + (len - full * a.c.page_size + T - 1) / T;
 }
-// the slot of a tile's first row and how many of its rows are live; the new token is a tile of its own, the last
+// the slot of a tile's first row and how many of its rows are live
 template <int T>
-__device__ __forceinline__ void attend_tile(const AttendArgs& a, int t, int n, int len, int& slot, int& valid, bool& is_new) {
-  is_new = a.nk1 != nullptr && t == n - 1;
-  if (is_new) {
-    slot = len; valid = 1;
-    return;
-  }
+__device__ __forceinline__ void attend_tile(const AttendArgs& a, int t, int len, int& slot, int& valid, bool& is_new) {
   slot = t * T;
   int end = len;
   if (a.tiles_per_page) {
     const int page = divide(t, a.tiles_per_page, a.tiles_magic);
     slot = page * a.c.page_size + (t - page * a.tiles_per_page) * T;
     end = min(len, (page + 1) * a.c.page_size);
+    is_new = t >= attend_tiles<T>(a, len);
+  } else {
+    is_new = slot >= len;
   }
   valid = min(T, end - slot);
+  if (is_new) {
+    slot = len;
+    valid = 1;
+  }
 }
 // A division of 64-bit numbers costs 0.25 us, and four of them stood in a row before the first load; nearly always 32 bits do.
 __device__ __forceinline__ long long quotient(long long n, long long d) {
@@ -197,7 +198,7 @@ diffattn_cache_attend_kernel(const __grid_constant__ CUtensorMap tm_k1, const __
   int sum = 0;
   for (int b = b0; b < b1; ++b) {
     const int len = cache_length(a.c, b);
-    sum += attend_tiles<T>(a, len);
+    sum += attend_tiles<T>(a, len) + (a.nk1 && (!a.counts || a.counts[b] > 0) ? 1 : 0);
     prefix[b + 1] = sum;
     length[b] = len;
     if (blockIdx.x == 0) {                     // for the joining kernel, which finds the lengths moved on
@@ -240,7 +241,7 @@ diffattn_cache_attend_kernel(const __grid_constant__ CUtensorMap tm_k1, const __
   auto look_up = [&](const TileWalk& w) {
     int slot, valid;
     bool is_new;
-    attend_tile<T>(a, w.t, w.n, w.len, slot, valid, is_new);
+    attend_tile<T>(a, w.t, w.len, slot, valid, is_new);
     Box x{-1, -1};
     if (!is_new && lane * a.box_rows < valid) {
       slot += lane * a.box_rows;
@@ -322,7 +323,7 @@ diffattn_cache_attend_kernel(const __grid_constant__ CUtensorMap tm_k1, const __
     }
     int slot, valid;
     bool is_new;
-    attend_tile<T>(a, cur.t, cur.n, cur.len, slot, valid, is_new);
+    attend_tile<T>(a, cur.t, cur.len, slot, valid, is_new);
     if (i == 0 || cur.t == 0) {
       // a (sequence, head) begins
       const int n = lane >> 2;
@@ -473,10 +474,12 @@ __device__ __forceinline__ Joined join_stats(const float4* stats, int first, int
   return j;
 }
 
-// What a call leaves behind besides y, for (sequence, head) bh; one thread.
-__device__ __forceinline__ void join_finish(const AttendArgs& a, int bh, int b, int head) {
+// What a call leaves behind besides y, for (sequence, head) bh of n tiles; one thread.
+template <int T>
+__device__ __forceinline__ void join_finish(const AttendArgs& a, int bh, int b, int head, int n) {
   if (a.nk1 == nullptr) return;
   const int len = a.length[b];
+  if (n <= attend_tiles<T>(a, len)) return;    // no token
   if (len < a.c.slots) {
     if (a.c.positions) a.c.positions[(size_t)bh * a.c.slots + len] = a.position[b];
     if (head == 0) {
@@ -516,7 +519,7 @@ __device__ __forceinline__ void join_weights(const AttendArgs& a, int bh, int sh
       if (tile >= n) continue;
       int slot, valid;
       bool is_new;
-      attend_tile<T>(a, tile, n, len, slot, valid, is_new);
+      attend_tile<T>(a, tile, len, slot, valid, is_new);
       if (row >= valid || slot + row >= a.c.slots) continue;
       at[k] = slot + row;
       s1[k] = scores[(long long)tile * 2 * T + row];
@@ -618,7 +621,7 @@ __global__ void __launch_bounds__(JT) diffattn_cache_join_kernel(const __grid_co
     }
   }
   if (threadIdx.x < 2 * D) a.y[size_t(bh) * 2 * D + threadIdx.x] = from_float16b<BF>(out * gain);
-  if (threadIdx.x == 0) join_finish(a, bh, b, head);
+  if (threadIdx.x == 0) join_finish<T>(a, bh, b, head, n);
 }
 
 template <int D, bool BF, bool TRACK>
@@ -684,7 +687,7 @@ __global__ void __launch_bounds__(JOIN_FEW) diffattn_cache_join_few_kernel(const
     const float g0 = a.gain ? a.gain[lane * C + k] : 1.f, g1 = a.gain ? a.gain[lane * C + k + 1] : 1.f;
     y[k / 2] = pack2<BF>(out[k] * g0, out[k + 1] * g1);
   }
-  if (lane == 0) join_finish(a, bh, b, head);
+  if (lane == 0) join_finish<T>(a, bh, b, head, n);
 }
 
 }  // namespace da

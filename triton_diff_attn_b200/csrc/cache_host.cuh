@@ -282,20 +282,22 @@ int diffattn_cache_attend(const DiffAttnCacheParams* p) {
     return fail(DIFFATTN_ERR_MISALIGNED, "lambda_scale or gain is not aligned to its type");
   const bool token = p->k1 || p->k2 || p->v;
   if (token && (rc = check_tokens(p, false))) return rc;
+  if (!aligned_to(p->counts, 4)) return fail(DIFFATTN_ERR_MISALIGNED, "counts is not 4-byte aligned");
   DeviceGuard guard;
   if ((rc = guard.enter(p->device))) return rc;
   const AttendSpace space = attend_space(p);
   if ((rc = check_cache_workspace(p, space.bytes))) return rc;
   if ((rc = cache_on_device(p))) return rc;
-  const void* dp[] = {p->q1, p->q2, p->lambda_scale, p->y, p->k1, p->k2, p->v, p->gain, p->workspace};
-  const char* dn[] = {"q1", "q2", "lambda_scale", "y", "k1", "k2", "v", "gain", "workspace"};
-  for (int i = 0; i < 9; ++i)
+  const void* dp[] = {p->q1, p->q2, p->lambda_scale, p->y, p->k1, p->k2, p->v, p->counts, p->gain, p->workspace};
+  const char* dn[] = {"q1", "q2", "lambda_scale", "y", "k1", "k2", "v", "counts", "gain", "workspace"};
+  for (int i = 0; i < 10; ++i)
     if ((rc = check_on_device(dp[i], p->device, dn[i]))) return rc;
   da::AttendArgs a;
   a.c = cache_args(p);
   a.q1 = static_cast<const uint4*>(p->q1); a.q2 = static_cast<const uint4*>(p->q2);
   a.q_b = pieces(p->q_stride_b, p->B > 1); a.q_h = pieces(p->q_stride_h, p->H > 1);
   a.nk1 = static_cast<const uint4*>(p->k1); a.nk2 = static_cast<const uint4*>(p->k2); a.nv = static_cast<const uint4*>(p->v);
+  a.counts = p->counts;
   a.nk_b = pieces(p->k_stride_b, p->B > 1); a.nk_h = pieces(p->k_stride_h, p->H > 1);
   a.nv_b = pieces(p->v_stride_b, p->B > 1); a.nv_h = pieces(p->v_stride_h, p->H > 1);
   a.scale_log2 = p->sm_scale * 1.4426950408889634f;

@@ -311,12 +311,13 @@ class DiffAttnCore(torch.nn.Module):
                                        dropout_p=self.dropout_p if self.training else 0.0, gain=self.gain)
 
     @torch.no_grad()
-    def decode(self, q1, q2, k1, k2, v, cache):
+    def decode(self, q1, q2, k1, k2, v, cache, counts=None):
         """One token of generation: stores the token's k1, k2 [B, H, 1, D] and v [B, H, 1, 2D] in `cache` (a `DiffAttnCache` that holds
         the tokens before it, the prompt's by `cache.append`) and returns its attention over all of them, [B, H, 1, 2D]: the last
-        row of what `forward` with causal=True gives for the whole sequence without dropout.  No gradients."""
+        row of what `forward` with causal=True gives for the whole sequence without dropout.  `counts`: as in `cache.attend`, for batches with
+        rows that are not in use.  No gradients."""
         lam = _core_lambda((self.lambda_q1, self.lambda_k1, self.lambda_q2, self.lambda_k2), self.lambda_init, getattr(q1, "device", None))
-        return cache.attend(q1, q2, lam, self.lambda_init, True, gain=self.gain, k1=k1, k2=k2, v=v)
+        return cache.attend(q1, q2, lam, self.lambda_init, True, gain=self.gain, k1=k1, k2=k2, v=v, counts=counts)
 
 
 def device_status(device=None) -> None:
