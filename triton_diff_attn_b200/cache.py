@@ -231,7 +231,7 @@ class DiffAttnCache:
 
     def append(self, k1, k2, v, counts=None) -> None:
         """Stores the tokens k1, k2 [B, H, T, D], v [B, H, T, 2D] behind each sequence's last one.  `counts` (an integer tensor [B]): sequence b
-        gets the first counts[b] of them (a padded batch; what lies behind is not read).  Their weights start at 0."""
+        gets the first counts[b] of them (a padded batch; what lies behind is not read).  Their weights start at 0, and only `attend` adds to them."""
         if not isinstance(k1, torch.Tensor) or k1.dim() != 4:
             raise (ValueError if isinstance(k1, torch.Tensor) else TypeError)("k1 must be a tensor [B, H, T, D]")
         p = self._params()
