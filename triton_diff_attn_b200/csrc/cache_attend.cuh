@@ -40,7 +40,7 @@ struct AttendArgs {
   int* prefix;                                 // [b + 2] tiles of the sequences before b, per head; at the end the workers that have any
   int* length;                                 // [b] cached tokens, before this call's
   int* position;                               // [b] the new token's position
-  float4* stats;                               // [workers + b * h] {m1, l1, m2, l2} of a piece
+  float4* stats;                               // [workers + b * h] {m1, l1, m2, l2} of a piece; m: what its exponents are taken from, near its maximum
   float4* acc;                                 // [workers + b * h][D] O1[2D], O2[2D] of a piece
   float* scores;                               // [tiles][2][T] (with weights)
 };
@@ -302,9 +302,14 @@ diffattn_cache_attend_kernel(const __grid_constant__ CUtensorMap tm_k1, const __
   // ---- the stretch.  With the rows r = 8 x matrix and columns c of the fragments as mma.sync lays them out:
   //  scores  S_b[16 tokens x 8] = K_b Q^T, Q^T's columns q1, q1, q2, q2, 0, 0, 0, 0: lane % 4 = 0 has S_1, lane % 4 = 1 has S_2 of tokens lane / 4
   //          and lane / 4 + 8, the other lanes nothing
-  //  P       a probability as two 16-bit numbers, its rounding and what that left out (bf16: 16 bits, fp16: 22), side by side in columns
-  //          2 b, 2 b + 1: transposed it is the operand of
+  //  P       a probability as two 16-bit numbers, its rounding and what that left out, side by side in columns 2 b, 2 b + 1: transposed it is the
+  //          operand of
   //  output  O^T[16 values x 8] += V^T P^T, columns O_1 (two shares), O_2 (two shares): the same lanes have the same branch
+  // What P loses: bf16 2^-17 of a probability.  fp16 has too few exponents for that in a long cache, where one token may be far above thousands that
+  // count together.  So its first number is kept 2^UP higher (the largest one between 2^7 and 2^15, where fp16 ends at 2^16) and its second one,
+  // which is 2^-11 of the first, 2^LOW higher again: off by 2^-22 of a probability, or 2^-43 of the largest one, whichever is more.
+  // (Without, 2^-25 of the largest: 16384 tokens of that size were lost from O but not from l.)
+  constexpr float UP = BF ? 0.f : 7.f, SLACK = 8.f, LOW = BF ? 1.f : 2048.f;
   const int branch = lane & 3;                 // 0, 1; 2 and 3: none
   const uint32_t row_k = smem_u32(ring) + (lane & 15) * G::K_ROW, row_v = smem_u32(ring) + 2 * G::K_BYTES + ((lane & 7) + ((lane >> 4) << 3)) * 128;
   const uint32_t sw_k = D == 32 ? ((lane >> 4) ^ ((lane >> 1) & 3)) << 4 : ((lane >> 4) ^ (lane & 7)) << 4, sw_v = (((lane >> 3) & 1) ^ (lane & 7)) << 4;
@@ -382,10 +387,10 @@ diffattn_cache_attend_kernel(const __grid_constant__ CUtensorMap tm_k1, const __
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-    // the running maximum moves only when it is exceeded by more than 2^8: the probabilities stay inside fp16's range either way
-    const bool need = top > m + 8.f;
+    // m, 2^UP below a maximum, moves only when that is exceeded by more than 2^SLACK: the probabilities stay inside fp16's range either way
+    const bool need = top > m + (UP + SLACK);
     if (__any_sync(0xffffffffu, need)) {
-      const float to = need ? top : m, f = ex2(m - to);
+      const float to = need ? top - UP : m, f = ex2(m - to);
       l *= f;
       m = to;
 #pragma unroll
@@ -401,7 +406,7 @@ diffattn_cache_attend_kernel(const __grid_constant__ CUtensorMap tm_k1, const __
         const float e = ex2(p[g][x] - m);
         l += e;
         const float hi = to_float16b<BF>(from_float16b<BF>(e));
-        pb[x] = movmatrix(pack2<BF>(hi, e - hi));
+        pb[x] = movmatrix(pack2<BF>(hi, (e - hi) * LOW));
       }
 #pragma unroll
       for (int k = 0; k < D / 8; ++k) {
@@ -430,8 +435,8 @@ diffattn_cache_attend_kernel(const __grid_constant__ CUtensorMap tm_k1, const __
         float* to = reinterpret_cast<float*>(a.acc + at * D) + branch * 2 * D + (lane >> 2);
 #pragma unroll
         for (int k = 0; k < D / 8; ++k) {
-          to[k * 16] = o[k][0] + o[k][1];
-          to[k * 16 + 8] = o[k][2] + o[k][3];
+          to[k * 16] = o[k][0] + o[k][1] * (1.f / LOW);
+          to[k * 16 + 8] = o[k][2] + o[k][3] * (1.f / LOW);
         }
       }
     }
@@ -443,7 +448,7 @@ diffattn_cache_attend_kernel(const __grid_constant__ CUtensorMap tm_k1, const __
 // ---------------------------------------------------------------------------------------------
 // Joins the pieces of every (sequence, head), and adds the tokens' weights.
 // ---------------------------------------------------------------------------------------------
-struct Joined { float m1, l1, m2, l2; };       // maximum and sum of both branches over all pieces
+struct Joined { float m1, l1, m2, l2; };       // the largest m and the sum of both branches over all pieces
 
 // the pieces of tiles [u, u + n) of the line: workers w0 .. w1
 __device__ __forceinline__ void piece_range(long long units, int workers, long long u, int n, int& w0, int& w1) {
