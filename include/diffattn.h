@@ -229,8 +229,9 @@ uint64_t diffattn_cache_workspace_bytes(const DiffAttnCacheParams* p, int32_t op
  * D1/D2 and dLambda partial buffers itself, src/kernel.py:522-529).  The forward needs none. */
 uint64_t diffattn_workspace_bytes(const DiffAttnParams* p);
 
-/* Synchronises `device` and reads the device-side status word: 0, or DIFFATTN_ERR_TIMEOUT with the
- * site in diffattn_last_error().  Clears the word.  (No counterpart in the reference.) */
+/* Synchronises `device` and reads the device-side status words: 0, or DIFFATTN_ERR_TIMEOUT with the
+ * site in diffattn_last_error(), or DIFFATTN_ERR_BAD_CACHE with what a cache's kernel met.  Clears the word it
+ * reports; where both are set the wait comes first and the next call reports the cache.  (No counterpart in the reference.) */
 int diffattn_status(int32_t device);
 
 const char* diffattn_last_error(void);   /* thread-local, never NULL */

@@ -3,20 +3,21 @@
 // A sequence's token j lies in slot j % page_size of page page_table[b][j / page_size]; a page holds the rows of all heads.  Rows: K1, K2 of
 // D, V of 2D 16-bit elements, 8 D bytes a token and head.  Nothing about a sequence is known on the host but the table's width, so lengths
 // and pages are checked here: a length outside [0, slots] counts as the nearest bound, a page outside the pool is not touched, and
-// both are reported through the status word.
+// both are reported through a status word of the cache's.
 #pragma once
 #include "sm100.cuh"
 
 namespace da {
 
-// what g_status[0] holds for a cache whose contents make no sense (sites of waits that gave up are below 900)
-constexpr int kCacheBadLength = 901, kCacheBadPage = 902, kCacheFull = 903;
+// A cache whose contents make no sense: what, sequence, where (the first report since diffattn_status last took one).  A word apart from g_status: a
+// full cache is the caller's doing and nothing unusual, and must not stand in the way of a wait that gives up later, in whatever kernel.
+__device__ int g_cache_status[3];
+constexpr int kCacheBadLength = 1, kCacheBadPage = 2, kCacheFull = 3;
 
-__device__ __noinline__ void cache_fault(int site, int b, int at) {
-  if (atomicCAS(&g_status[0], 0, site) == 0) {
-    g_status[1] = b;
-    g_status[2] = at;
-    g_status[3] = 0;
+__device__ __noinline__ void cache_fault(int what, int b, int at) {
+  if (atomicCAS(&g_cache_status[0], 0, what) == 0) {
+    g_cache_status[1] = b;
+    g_cache_status[2] = at;
   }
 }
 

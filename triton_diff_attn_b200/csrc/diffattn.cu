@@ -666,10 +666,16 @@ int diffattn_status(int32_t device) {
   if (st[0] != 0) {
     int zero[4] = {0, 0, 0, 0};
     cudaMemcpyToSymbol(da::g_status, zero, sizeof(zero));
-    if (st[0] == da::kCacheBadLength) return fail(DIFFATTN_ERR_BAD_CACHE, "cache: sequence %d has length %d", st[1], st[2]);
-    if (st[0] == da::kCacheBadPage) return fail(DIFFATTN_ERR_BAD_CACHE, "cache: entry %d of sequence %d's page table is no page of the pool", st[2], st[1]);
-    if (st[0] == da::kCacheFull) return fail(DIFFATTN_ERR_BAD_CACHE, "cache: sequence %d is full (length %d), tokens were dropped", st[1], st[2]);
     return fail(DIFFATTN_ERR_TIMEOUT, "device-side wait gave up at site %d (block %d,%d iteration %d)", st[0], st[1], st[2], st[3]);
+  }
+  int cs[3] = {0, 0, 0};
+  DA_CUDA(cudaMemcpyFromSymbol(cs, da::g_cache_status, sizeof(cs)));
+  if (cs[0] != 0) {
+    int zero[3] = {0, 0, 0};
+    cudaMemcpyToSymbol(da::g_cache_status, zero, sizeof(zero));
+    if (cs[0] == da::kCacheBadLength) return fail(DIFFATTN_ERR_BAD_CACHE, "cache: sequence %d has length %d", cs[1], cs[2]);
+    if (cs[0] == da::kCacheBadPage) return fail(DIFFATTN_ERR_BAD_CACHE, "cache: entry %d of sequence %d's page table is no page of the pool", cs[2], cs[1]);
+    return fail(DIFFATTN_ERR_BAD_CACHE, "cache: sequence %d is full (length %d), tokens were dropped", cs[1], cs[2]);
   }
   return DIFFATTN_OK;
 }

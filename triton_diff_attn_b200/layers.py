@@ -321,6 +321,7 @@ class DiffAttnCore(torch.nn.Module):
 
 
 def device_status(device=None) -> None:
-    """Synchronise and raise RuntimeError if a device-side bounded wait gave up in any kernel."""
+    """Synchronise and raise RuntimeError if a device-side bounded wait gave up in any kernel, ValueError if a kernel of a `DiffAttnCache` met a
+    length, a page or a full sequence that it could not use.  Each is reported once; a wait that gave up first."""
     dev = torch.cuda.current_device() if device is None else torch.device(device).index
     _lib.check(_lib.lib.diffattn_status(int(dev)), "diffattn_status")
