@@ -1,0 +1,56 @@
+"""What `DiffAttnCache` makes of its arguments before anything is launched (no GPU: a library that only writes down what it is given)."""
+import ctypes
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from triton_diff_attn_b200 import _lib, cache as cache_module
+
+
+class _Library:
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        def call(p, *rest):
+            if name != "diffattn_cache_workspace_bytes":
+                self.calls.append((name, _lib.DiffAttnCacheParams.from_buffer_copy(p)))
+            return 0
+        return call
+
+
+@pytest.fixture
+def bare(monkeypatch):
+    """A cache of 2 sequences, 3 heads, D = 64 and 64 slots without memory, and its library."""
+    library = _Library()
+    monkeypatch.setattr(cache_module, "_lib", SimpleNamespace(**{**vars(_lib), "lib": library}))
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 0, raising=False)
+    c = cache_module.DiffAttnCache.__new__(cache_module.DiffAttnCache)
+    p = _lib.DiffAttnCacheParams()
+    p.struct_size = ctypes.sizeof(p)
+    p.B, p.H, p.D, p.page_size, p.num_pages, p.max_pages = 2, 3, 64, 16, 9, 4
+    c._sizes, c._shape, c._device, c._index, c._dtype = p, (2, 3, 64), torch.device("cpu"), -1, torch.float16
+    c._lengths, c._y, c._attend_bytes = torch.zeros(2, dtype=torch.int32), torch.empty(2, 3, 1, 128, dtype=torch.float16), 0
+    c._counter = torch.zeros(1, dtype=torch.int32)
+    return c, library.calls
+
+
+@pytest.mark.parametrize("keep,recent,error", [
+    (2 ** 32 + 5, 0, ValueError), (-2 ** 32 + 5, 0, ValueError), (5, 2 ** 32, ValueError), (5, -2 ** 32 + 1, ValueError), (65, 0, ValueError), (0, 0, ValueError),
+    (5, 6, ValueError), (5, -1, ValueError), (40.9, 0, TypeError), (40, 1.5, TypeError), ("40", 0, TypeError), (None, 0, TypeError),
+])
+def test_evict_refuses_sizes(bare, keep, recent, error):
+    c, calls = bare
+    with pytest.raises(error):
+        c.evict(keep, recent)
+    assert not calls
+
+
+def test_evict_takes_whole_numbers(bare):
+    np = pytest.importorskip("numpy")
+    c, calls = bare
+    for keep, recent in ((40, 7), (np.int64(40), np.int32(7)), (torch.tensor(40), torch.tensor(7)), (64, 64), (1, 0)):
+        c.evict(keep, recent)
+        name, p = calls.pop()
+        assert (name, p.keep, p.recent) == ("diffattn_cache_evict", int(keep), int(recent)) and not calls

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import operator
 
 import torch
 
@@ -296,8 +297,11 @@ class DiffAttnCache:
         the largest `weights` (ties: the lowest slot); without weights those of the largest positions.  `evict(n, recent=n)` is a window of the
         last n tokens.  Survivors move into the slots that come free, so tokens change their slots (`positions` says which is where).
         Pages behind the new lengths are free again."""
+        keep, recent = operator.index(keep), operator.index(recent)      # (a field of 32 bits would take the lowest ones of any number)
+        if not (1 <= keep <= self.slots and 0 <= recent <= keep):
+            raise ValueError(f"keep={keep} must lie in [1, {self.slots}], recent={recent} in [0, keep]")
         p = self._params()
-        p.keep, p.recent = int(keep), int(recent)
+        p.keep, p.recent = keep, recent
         nbytes = int(_lib.lib.diffattn_cache_workspace_bytes(p, _lib.CACHE_EVICT))
         ws = self._workspace(p, nbytes) if nbytes else None  # noqa: F841
         _lib.check(_lib.lib.diffattn_cache_evict(p), "diffattn_cache_evict")
