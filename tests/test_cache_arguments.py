@@ -54,3 +54,59 @@ def test_evict_takes_whole_numbers(bare):
         c.evict(keep, recent)
         name, p = calls.pop()
         assert (name, p.keep, p.recent) == ("diffattn_cache_evict", int(keep), int(recent)) and not calls
+
+
+def _tensors():
+    r = lambda *shape: torch.ones(shape, dtype=torch.float16)
+    return dict(q1=r(2, 3, 1, 64), q2=r(2, 3, 1, 64), lambda_scale=torch.full((1,), 0.5), gain=torch.ones(128), k1=r(2, 3, 1, 64), k2=r(2, 3, 1, 64), v=r(2, 3, 1, 128))
+
+
+@pytest.mark.parametrize("name", list(_tensors()))
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_tangents_are_refused(bare, name, grad):
+    """y would come back without one.  (no_grad does not switch forward mode off.)"""
+    import torch.autograd.forward_ad as fw
+    c, calls = bare
+    with fw.dual_level(), torch.set_grad_enabled(grad):
+        t = _tensors()
+        c.attend(**t)                                     # a level alone is no tangent
+        c.append(t["k1"], t["k2"], t["v"])
+        assert [n for n, _ in calls] == ["diffattn_cache_attend", "diffattn_cache_append"]
+        t[name] = fw.make_dual(t[name], torch.ones_like(t[name]))
+        with pytest.raises(NotImplementedError, match=name):
+            c.attend(**t)
+        if name in ("k1", "k2", "v"):
+            with pytest.raises(NotImplementedError, match=name):
+                c.append(t["k1"], t["k2"], t["v"])
+        assert len(calls) == 2
+    with fw.dual_level(), torch.inference_mode():         # (this does)
+        c.attend(**t)
+    assert len(calls) == 3
+
+
+def test_decode_refuses_tangents(bare):
+    import torch.autograd.forward_ad as fw
+    from triton_diff_attn_b200 import DiffAttnCore
+    c, calls = bare
+    core, t = DiffAttnCore(64, causal=True), _tensors()
+    rows = [t[n] for n in ("q1", "q2", "k1", "k2", "v")]
+    core.decode(*rows, c)
+    with fw.dual_level():
+        for i in range(5):
+            with pytest.raises(NotImplementedError):
+                core.decode(*(fw.make_dual(x, x) if i == j else x for j, x in enumerate(rows)), c)
+        for n in ("lambda_q1", "gain"):
+            p = dict(core.named_parameters())[n]
+            dual = {n: fw.make_dual(p.detach(), torch.ones_like(p))}
+            with pytest.raises(NotImplementedError):
+                torch.func.functional_call(_Decode(core), {"core." + k: x for k, x in dual.items()}, (rows, c))
+    assert len(calls) == 1
+
+
+class _Decode(torch.nn.Module):
+    def __init__(self, core):
+        super().__init__()
+        self.core = core
+
+    def forward(self, rows, cache):
+        return self.core.decode(*rows, cache)

@@ -12,6 +12,7 @@ import math
 import operator
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .layers import _IO_DTYPES, _LAMBDA_DTYPES, EPS
@@ -42,6 +43,13 @@ def _pair(a, b):
         a, b = a.clone(memory_format=torch.contiguous_format), b.clone(memory_format=torch.contiguous_format)
         sa = a.stride()
     return a, b, sa
+
+
+def _refuse_tangents(**tensors):
+    """Inside a level of forward-mode differentiation (the caller looks for one first): what comes out here would have lost a tangent."""
+    for name, t in tensors.items():
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{name} has a forward-mode tangent, and the cache has no derivatives")
 
 
 class DiffAttnCache:
@@ -135,6 +143,8 @@ class DiffAttnCache:
                 raise RuntimeError(f"{name} is on {t.device}, k1_pages on {device}")
             if t is not None and t.requires_grad:
                 raise ValueError(f"{name} requires a gradient: the cache has no backward pass")
+            if forward_ad._current_level >= 0:
+                _refuse_tangents(**{name: t})
         self._k1_pages, self._k2_pages, self._v_pages, self._page_table = k1_pages, k2_pages, v_pages, page_table
         self._lengths, self._positions, self._next_position, self._weights = lengths, positions, next_position, weights
         self._counter = lengths.new_zeros(1)      # every writing call leaves it 0
@@ -201,6 +211,8 @@ class DiffAttnCache:
         self._check("k1", k1, rows, d)
         self._check("k2", k2, rows, d)
         self._check("v", v, rows, 2 * d)
+        if forward_ad._current_level >= 0:
+            _refuse_tangents(k1=k1, k2=k2, v=v)
         k1, k2, sk = _pair(k1, k2)
         v, sv = _rows(v)
         p.k1, p.k2, p.v = k1.data_ptr(), k2.data_ptr(), v.data_ptr()
@@ -264,6 +276,8 @@ class DiffAttnCache:
                 raise ValueError("gain must be a floating-point tensor of shape [2*D] on the cache's device")
         if (lam.requires_grad or (gain is not None and gain.requires_grad)) and torch.is_grad_enabled():
             raise RuntimeError("lambda_scale or gain requires a gradient, and the cache has no backward pass: call it under torch.no_grad()")
+        if forward_ad._current_level >= 0:
+            _refuse_tangents(q1=q1, q2=q2, lambda_scale=lam, gain=gain)
         p = self._params()
         if k1 is not None or k2 is not None or v is not None:
             keep = self._tokens(p, k1, k2, v, 1)  # noqa: F841  (copies stay until the call is enqueued)
