@@ -171,7 +171,7 @@ int diffattn_lambda_bwd(int32_t device, void* stream, int32_t n, const float* q1
  * outside [0, num_pages) is neither read nor written, tokens that do not fit are dropped; the results of such a call are undefined,
  * and diffattn_status reports it as DIFFATTN_ERR_BAD_CACHE.  Pages may be shared between sequences (a common prefix) as long as the slots
  * that a call writes belong to one sequence: the one behind each length (append, attend with a token), all of a sequence longer than
- * `keep` (evict).  B <= 4096, B * H <= 65535, slots + max(page_size, 64) < 2^31.  Calls are enqueued on `stream`, allocate nothing and can be captured. */
+ * `keep` (evict).  B <= 4096, B * H <= 65535, slots + max(page_size, 7936) < 2^31 (head dim 32 in pages of one: slots < 2^31 - 2^17).  Calls are enqueued on `stream`, allocate nothing and can be captured. */
 typedef struct DiffAttnCacheParams {
   uint32_t struct_size;            /* sizeof(DiffAttnCacheParams) */
   int32_t device;

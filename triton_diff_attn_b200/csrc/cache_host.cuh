@@ -80,9 +80,11 @@ int check_cache_sizes(const DiffAttnCacheParams* p) {
     return fail(DIFFATTN_ERR_BAD_SHAPE, "B=%d H=%d: B <= %d and B*H <= 65535", p->B, p->H, da::attend::MAX_B);
   if (p->page_size <= 0 || p->num_pages <= 0 || p->max_pages <= 0)
     return fail(DIFFATTN_ERR_BAD_SHAPE, "page_size=%d num_pages=%d max_pages=%d must be positive", p->page_size, p->num_pages, p->max_pages);
-  // (the kernels add a page or two tiles to a slot in 32 bits)
-  if ((long long)p->max_pages * p->page_size + std::max(p->page_size, 64) > INT32_MAX || most_tiles(p) * std::max(p->B, 1) > INT32_MAX ||
-      most_tiles(p) * std::max(p->B, 1) * std::max(p->H, 1) > (1ll << 39))
+  // In 32 bits the kernels add to a slot: a page, two tiles, a round of the selection's loads or runs.  To a tile: a round of all
+  // shares that add weights, 4 x 64 tiles each.
+  constexpr int slot_step = std::max(2 * da::SELECT_THREADS * da::SELECT_AHEAD, 31 * da::SELECT_THREADS), tile_step = 1 << 17;
+  if ((long long)p->max_pages * p->page_size + std::max(p->page_size, slot_step) > INT32_MAX || most_tiles(p) + tile_step > INT32_MAX ||
+      most_tiles(p) * std::max(p->B, 1) > INT32_MAX || most_tiles(p) * std::max(p->B, 1) * std::max(p->H, 1) > (1ll << 39))
     return fail(DIFFATTN_ERR_BAD_SHAPE, "max_pages=%d of %d slots: too long", p->max_pages, p->page_size);
   return DIFFATTN_OK;
 }
