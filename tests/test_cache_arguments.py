@@ -110,3 +110,25 @@ class _Decode(torch.nn.Module):
 
     def forward(self, rows, cache):
         return self.core.decode(*rows, cache)
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_counts_beyond_32_bits(bare, monkeypatch, dtype):
+    """More than there are rows means all of them, less than none means none, whatever the number."""
+    c, _ = bare
+    seen = []
+    read = lambda p, *_: seen.append(list((ctypes.c_int32 * 2).from_address(p.counts))) or 0
+    monkeypatch.setattr(cache_module._lib.lib, "diffattn_cache_append", read, raising=False)
+    monkeypatch.setattr(cache_module._lib.lib, "diffattn_cache_attend", read, raising=False)
+    t = _tensors()
+    rows = [torch.ones(2, 3, 5, w, dtype=torch.float16) for w in (64, 64, 128)]
+    far = [2 ** 32, 2 ** 32 + 3, 2 ** 31, -2 ** 32 + 2, -2 ** 63, 2 ** 63 - 1] if dtype == torch.int64 else [2 ** 31 - 1, -2 ** 31]
+    for n in far + [0, 1, 3, 5, 6, -1]:
+        counts = torch.tensor([n, 2], dtype=dtype)
+        c.append(*rows, counts)
+        a, b = seen.pop()
+        assert (min(max(a, 0), 5), b) == (min(max(n, 0), 5), 2)      # (the kernels clamp what they get)
+        c.attend(**t, counts=counts)
+        a, b = seen.pop()
+        assert (a > 0, b > 0) == (n > 0, True)
+        assert counts.tolist() == [n, 2]

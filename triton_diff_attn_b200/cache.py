@@ -220,15 +220,16 @@ class DiffAttnCache:
         p.v_stride_b, p.v_stride_h, p.v_stride_t, _ = sv
         return k1, k2, v
 
-    def _counts(self, p, counts):
+    def _counts(self, p, counts, most):
         if not isinstance(counts, torch.Tensor):
             raise TypeError("counts must be a tensor")
         if counts.get_device() != self._index:
             raise RuntimeError(f"counts is on {counts.device}, the cache on {self._device}")
         if counts.dtype not in (torch.int32, torch.int64) or tuple(counts.shape) != (self._shape[0],):
             raise ValueError(f"counts must be int32 or int64 of shape {(self._shape[0],)}")
-        if counts.dtype is not torch.int32 or not counts.is_contiguous():
-            counts = counts.to(torch.int32).contiguous()
+        if counts.dtype is not torch.int32:
+            counts = counts.clamp(0, most).to(torch.int32)      # (not the lowest 32 bits of whatever it is)
+        counts = counts.contiguous()
         p.counts = counts.data_ptr()
         return counts
 
@@ -244,14 +245,15 @@ class DiffAttnCache:
 
     def append(self, k1, k2, v, counts=None) -> None:
         """Stores the tokens k1, k2 [B, H, T, D], v [B, H, T, 2D] behind each sequence's last one.  `counts` (an integer tensor [B]): sequence b
-        gets the first counts[b] of them (a padded batch; what lies behind is not read).  Their weights start at 0, and only `attend` adds to them."""
+        gets the first counts[b] of them, all where there are not so many (a padded batch; what lies behind is not read).
+        Their weights start at 0, and only `attend` adds to them."""
         if not isinstance(k1, torch.Tensor) or k1.dim() != 4:
             raise (ValueError if isinstance(k1, torch.Tensor) else TypeError)("k1 must be a tensor [B, H, T, D]")
         p = self._params()
         p.T = k1.shape[2]
         keep = self._tokens(p, k1, k2, v, p.T)  # noqa: F841  (copies stay until the call is enqueued)
         if counts is not None:
-            counts = self._counts(p, counts)
+            counts = self._counts(p, counts, p.T)
         _lib.check(_lib.lib.diffattn_cache_append(p), "diffattn_cache_append")
 
     def attend(self, q1, q2, lambda_scale, lambda_init: float = 0.8, rms_norm: bool = False, gain=None, k1=None, k2=None, v=None,
@@ -282,7 +284,7 @@ class DiffAttnCache:
         if k1 is not None or k2 is not None or v is not None:
             keep = self._tokens(p, k1, k2, v, 1)  # noqa: F841  (copies stay until the call is enqueued)
             if counts is not None:
-                counts = self._counts(p, counts)
+                counts = self._counts(p, counts, 1)
         elif counts is not None:
             raise ValueError("counts goes with a token: k1, k2 and v are missing")
         q1, q2, sq = _pair(q1, q2)
