@@ -1,0 +1,50 @@
+"""The key-value cache's tensors and contents that a user can hand over, and what must not come of them."""
+import math
+
+import pytest
+import torch
+
+from test_cache_gpu import DEV, make, queries, snapshot
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def pkg():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    import triton_diff_attn_b200
+    return triton_diff_attn_b200
+
+
+def test_a_cache_made_in_a_capture(pkg):
+    """Calls on it outside the graph, before its first replay and after, move the lengths on as those in the graph do."""
+    c0 = make(pkg, [5, 20], 2, 64, 16, track=True, room=28, seed=1)
+    state = (c0.k1_pages, c0.k2_pages, c0.v_pages, c0.page_table, c0.lengths)
+    more = dict(positions=c0.positions, next_position=c0.next_position, weights=c0.weights)
+    q1, q2, k1, k2, v = queries(2, 2, 64, torch.float16, seed=1)
+    c0.append(k1, k2, v)
+    torch.cuda.synchronize()
+    pool = torch.cuda.graph_pool_handle()
+    soil = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(soil, pool=pool):              # what lies in the graphs' memory is not 0
+        dirt = [torch.full((64,), 7, dtype=torch.int32, device=DEV) for _ in range(64)]
+    soil.replay()
+    torch.cuda.synchronize()
+    del dirt
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, pool=pool):
+        c = pkg.DiffAttnCache.from_tensors(*state, **more)
+        c.append(k1, k2, v)
+        c.evict(18)
+    assert c.lengths.tolist() == [6, 21]
+    for eager in (True, False, True, False):
+        c.lengths.copy_(torch.tensor([6, 18], dtype=torch.int32))
+        if eager:
+            c.append(k1, k2, v)
+            assert c.lengths.tolist() == [7, 19]
+            c.evict(18)
+        else:
+            graph.replay()
+        assert c.lengths.tolist() == [7, 18]
+    pkg.device_status(0)

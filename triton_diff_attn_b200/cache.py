@@ -147,8 +147,11 @@ class DiffAttnCache:
                 _refuse_tangents(**{name: t})
         self._k1_pages, self._k2_pages, self._v_pages, self._page_table = k1_pages, k2_pages, v_pages, page_table
         self._lengths, self._positions, self._next_position, self._weights = lengths, positions, next_position, weights
-        self._counter = lengths.new_zeros(1)      # every writing call leaves it 0
-        if not torch.cuda.is_current_stream_capturing():
+        # What append and evict count their CTAs with: 0 between calls, every one of them leaves it so.  Made in a capture it would be 0
+        # in that graph's replays only, so a cache made there takes a new one for every call.
+        with torch.cuda.device(device):
+            self._counter = None if torch.cuda.is_current_stream_capturing() else lengths.new_zeros(1)
+        if self._counter is not None:
             torch.cuda.current_stream(device).synchronize()      # (the first call may come on another stream)
         self._shape = (batch, heads, d)
         self._device, self._index, self._dtype = device, k1_pages.get_device(), k1_pages.dtype
@@ -163,8 +166,9 @@ class DiffAttnCache:
         p.table_stride = page_table.stride(0)
         p.sm_scale, p.eps = 1.0 / math.sqrt(d), EPS
         # the tensors stay where they are for the cache's life (and their memory with it, whatever becomes of the tensor objects)
-        p.k1_pages, p.k2_pages, p.v_pages, p.page_table, p.lengths, p.counter = (t.data_ptr() for t in (
-            k1_pages, k2_pages, v_pages, page_table, lengths, self._counter))
+        p.k1_pages, p.k2_pages, p.v_pages, p.page_table, p.lengths = (t.data_ptr() for t in (k1_pages, k2_pages, v_pages, page_table, lengths))
+        if self._counter is not None:
+            p.counter = self._counter.data_ptr()
         if positions is not None:
             p.positions, p.next_position = positions.data_ptr(), next_position.data_ptr()
         if weights is not None:
@@ -233,6 +237,14 @@ class DiffAttnCache:
         p.counts = counts.data_ptr()
         return counts
 
+    def _count_with(self, p):
+        """The counter of a call that writes, where the cache has none of its own; to be kept until the call is enqueued."""
+        if self._counter is not None:
+            return None
+        counter = self._lengths.new_zeros(1)
+        p.counter = counter.data_ptr()
+        return counter
+
     def _workspace(self, p, nbytes):
         ws = self._lengths.new_empty(max(nbytes, 256) // 4)
         p.workspace, p.workspace_bytes = ws.data_ptr(), nbytes
@@ -254,6 +266,7 @@ class DiffAttnCache:
         keep = self._tokens(p, k1, k2, v, p.T)  # noqa: F841  (copies stay until the call is enqueued)
         if counts is not None:
             counts = self._counts(p, counts, p.T)
+        counter = self._count_with(p)  # noqa: F841
         _lib.check(_lib.lib.diffattn_cache_append(p), "diffattn_cache_append")
 
     def attend(self, q1, q2, lambda_scale, lambda_init: float = 0.8, rms_norm: bool = False, gain=None, k1=None, k2=None, v=None,
@@ -320,4 +333,5 @@ class DiffAttnCache:
         p.keep, p.recent = keep, recent
         nbytes = int(_lib.lib.diffattn_cache_workspace_bytes(p, _lib.CACHE_EVICT))
         ws = self._workspace(p, nbytes) if nbytes else None  # noqa: F841
+        counter = self._count_with(p)  # noqa: F841
         _lib.check(_lib.lib.diffattn_cache_evict(p), "diffattn_cache_evict")
