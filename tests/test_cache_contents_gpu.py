@@ -48,3 +48,21 @@ def test_a_cache_made_in_a_capture(pkg):
             graph.replay()
         assert c.lengths.tolist() == [7, 18]
     pkg.device_status(0)
+
+
+def test_state_that_shares_memory_is_refused(pkg):
+    """`append` would count twice what is both a length and a next position."""
+    c = make(pkg, [5, 20], 2, 64, 16, track=True, room=4)
+    pools = (c.k1_pages, c.k2_pages, c.v_pages, c.page_table)
+    take = pkg.DiffAttnCache.from_tensors
+    both = torch.zeros(3, dtype=torch.int32, device=DEV)
+    for lengths, following, positions, weights in (
+            (c.lengths, c.lengths, c.positions, None), (both[:2], both[1:], c.positions, None),
+            (c.lengths, c.positions.view(-1)[:2], c.positions, None), (c.lengths, c.next_position, c.positions, c.positions.view(torch.float32))):
+        with pytest.raises(ValueError, match="share memory"):
+            take(*pools, lengths, positions=positions, next_position=following, weights=weights)
+    state = torch.zeros(4, dtype=torch.int32, device=DEV)      # neighbours do not
+    take(*pools, state[:2], positions=c.positions, next_position=state[2:], weights=c.weights).reset()
+    empty = torch.zeros(0, dtype=torch.int32, device=DEV)
+    take(*pools[:3], c.page_table[:0], empty, positions=c.positions[:0], next_position=empty)
+    pkg.device_status(0)

@@ -127,6 +127,7 @@ class DiffAttnCache:
         slots = max_pages * page_size
         if (positions is None) != (next_position is None):
             raise ValueError("positions and next_position go together")
+        spans = []
         for name, t, shape, dtype in (("lengths", lengths, (batch,), torch.int32), ("next_position", next_position, (batch,), torch.int32),
                                       ("positions", positions, (batch, heads, slots), torch.int32),
                                       ("weights", weights, (batch, heads, slots), torch.float32)):
@@ -136,6 +137,12 @@ class DiffAttnCache:
                 raise TypeError(f"{name} must be a tensor")
             if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
                 raise ValueError(f"{name} must be {dtype} {shape}, contiguous")
+            if t.is_cuda and t.numel():
+                spans.append((t.data_ptr(), t.data_ptr() + 4 * t.numel(), name))
+        spans.sort()
+        for (_, end, a), (start, _, b) in zip(spans, spans[1:]):
+            if start < end:
+                raise ValueError(f"{a} and {b} share memory")
         device = k1_pages.device
         for name, t in pools + (("page_table", page_table), ("lengths", lengths), ("positions", positions), ("next_position", next_position),
                                 ("weights", weights)):
