@@ -66,3 +66,13 @@ def test_state_that_shares_memory_is_refused(pkg):
     empty = torch.zeros(0, dtype=torch.int32, device=DEV)
     take(*pools[:3], c.page_table[:0], empty, positions=c.positions[:0], next_position=empty)
     pkg.device_status(0)
+
+
+def test_a_page_table_wider_than_32_bits_is_refused(pkg):
+    """It would be taken for one of as many columns as its lowest 32 bits say."""
+    pools = tuple(torch.zeros(2, 1, 16, w, dtype=torch.float16, device=DEV) for w in (64, 64, 128))
+    none = torch.zeros(0, dtype=torch.int32, device=DEV)
+    for columns in (2 ** 32 + 4, 2 ** 31, 2 ** 27):      # (the last: too many slots)
+        with pytest.raises(ValueError, match="too long"):
+            pkg.DiffAttnCache.from_tensors(*pools, none.new_empty(0, columns), none)
+    assert pkg.DiffAttnCache.from_tensors(*pools, none.new_empty(0, 4), none).slots == 64

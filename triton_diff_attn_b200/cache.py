@@ -125,6 +125,8 @@ class DiffAttnCache:
         if batch > 1 and page_table.stride(0) < max_pages:
             raise ValueError("the rows of page_table must not overlap")
         slots = max_pages * page_size
+        if max(slots, pages, heads, batch) >= 2 ** 31:      # (the library's fields; it has closer limits of its own)
+            raise ValueError(f"{batch} sequences of {max_pages} pages of {page_size} slots, {pages} pages, {heads} heads: too long for 32 bits")
         if (positions is None) != (next_position is None):
             raise ValueError("positions and next_position go together")
         spans = []
