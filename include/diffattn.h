@@ -164,8 +164,8 @@ int diffattn_lambda_bwd(int32_t device, void* stream, int32_t n, const float* q1
  * lengths [B]: tokens that each sequence holds, in slots 0 .. lengths[b] - 1; 0 is a sequence that is not in use.  next_position [B]: tokens
  * it has had.  positions [B][H][slots]: the position of the token in each slot (per head: heads lose different tokens).  weights
  * [B][H][slots]: the attention weight that each token has gathered, sum of |P_1 - lambda P_2| over the queries that saw it.  positions and
- * next_position go together; they and weights may be NULL where nothing is evicted.  Slots behind a sequence's length are never
- * read, and written only by append.
+ * next_position go together; they and weights may be NULL where nothing is evicted.  What lies in slots behind a
+ * sequence's length never reaches a result; they are written only by append and, the one at the length, by attend with a token.
  *
  * Lengths and pages lie on the device, so the kernels check them: a length outside [0, slots] counts as the nearest bound, a page
  * outside [0, num_pages) is neither read nor written, tokens that do not fit are dropped; the results of such a call are undefined,
