@@ -50,10 +50,11 @@ AttendSpace attend_space(const DiffAttnCacheParams* p) {
 }
 int evict_most(const DiffAttnCacheParams* p) { return std::min(p->keep, p->max_pages * p->page_size - p->keep); }
 
-// The selecting kernel moves rows itself where they are few a CTA, or there are CTAs for every SM.  Appending and evicting at D 64 with and without the
-// second kernel, us: B8 H16, 512 of 4608 slots 35 / 48; B16 H16, 256 of 2304 33 / 36; B32 H16, 128 of 1152 34 / 32; B64 H16, 8 of up to 512 20 / 18;
-// B16 H16, one of up to 1025 15 / 13.
-bool evict_at_once(const DiffAttnCacheParams* p) { return evict_most(p) <= 64 || p->B * p->H >= sm_count(p->device); }
+// The selecting kernel moves rows itself where they are few a CTA (one launch less), or there are three CTAs and more for every SM, whose moves and
+// selections then overlap.  Appending a chunk and evicting as many tokens at D 64 with the second kernel / without, us: 512 moves, 16 CTAs
+// 20 / 39, 128 CTAs 34 / 46; 256 moves, 160 CTAs 24 / 28, 256 CTAs 33 / 36, 384 CTAs 46.7 / 47.7; 1024 moves, 256 CTAs 104 / 133, 512 CTAs 194 / 192;
+// 128 moves, 64 CTAs 16 / 20, 512 CTAs 34 / 31; 64 moves, 64 CTAs 15.2 / 14.5, 256 CTAs 14.8 / 14.5, 1024 CTAs 38 / 36.
+bool evict_at_once(const DiffAttnCacheParams* p) { return evict_most(p) <= 64 || p->B * p->H >= 3 * sm_count(p->device); }
 struct EvictSpace {
   uint64_t moves, bytes;
 };
@@ -182,7 +183,10 @@ int attend_launch(const DiffAttnCacheParams* p, da::AttendArgs& a) {
   const cudaStream_t stream = static_cast<cudaStream_t>(p->stream);
   const int sms = sm_count(p->device);
   if ((rc = launch(kernel, dim3(sms), da::attend::Geo<D>::THREADS, smem, stream, true, k1, k2, v, a))) return rc;
-  // How many pieces a (sequence, head) has goes by how many of them share the workers, and by its tiles.
+  // How many pieces a (sequence, head) has goes by how many of them share the workers, and by its tiles.  Whole calls at D 64 without weights, us, joined
+  // by 1024 threads / 256 / a warp: 65 pieces (B1 H16 N8192) 19.5 / 22.0 / 38; 40 (H26 N4096) 17.8 / 18.4 / 29; 22 (B2 H24) 24.6 / 24.0 / 31; 16 (B4
+  // H16) 30.0 / 29.0 / 34; 4 (B16 H16 N1024) 34.2 / 29.4 / 30.8; 3 (340 heads) 43.5 / 36.8 / 36.9; 2 (384 heads) 47.3 / 40.5 / 40.1; 1 (B64 H16) 110 / 90 / 88.
+  // (By the batch's capacity, not by the sequences in use, which the host does not know: few long ones in a large batch are joined slowly.)
   const int bh = p->B * p->H;
   const long long pieces = std::min((long long)a.workers / bh, most_tiles(p));
   auto weights = [&](int blocks) { return TRACK ? bh * ((blocks + bh - 1) / bh) : 0; };
