@@ -334,8 +334,8 @@ class DiffAttnCache:
         """Cuts every sequence longer than `keep` back to `keep` tokens, per head: the tokens of its last `recent` positions stay, then those with
         the largest `weights` (ties: the lowest slot); without weights those of the largest positions.  `evict(n, recent=n)` is a window of the
         last n tokens.  Weights are what `attend` has added since a token was stored: right behind a prompt's `append` they are all 0, and but for `recent`
-        the oldest tokens stay; a few steps later they rank tokens by those steps.  Survivors move into the slots that come free, so tokens change their slots (`positions` says which is where).
-        Pages behind the new lengths are free again."""
+        the oldest tokens stay; a few steps later they rank tokens by those steps.  Survivors move into the slots that come free, so tokens change
+        their slots (`positions` says which is where).  Pages behind the new lengths are free again."""
         keep, recent = operator.index(keep), operator.index(recent)      # (a field of 32 bits would take the lowest ones of any number)
         if not (1 <= keep <= self.slots and 0 <= recent <= keep):
             raise ValueError(f"keep={keep} must lie in [1, {self.slots}], recent={recent} in [0, keep]")
